@@ -1,5 +1,6 @@
-"""Measured cases of the language-model tuning operators: scaled embedding lookup and its gradient, the clipped policy
-loss and the paired preference loss with their logit gradients, and the global gradient norm with clipping.
+"""Measured cases of the language-model tuning operators: scaled embedding lookup and its gradient, token
+log-probabilities, the clipped policy loss and the paired preference loss with their logit gradients, and the global
+gradient norm with clipping.
 
 ``run(state)`` makes one pass.  With ``own`` false it evaluates the formula in elementary torch operations in 32 bits,
 rounded once at the end; with ``own`` true it makes the call a user of the package makes.  ``exact`` restates the
@@ -40,18 +41,16 @@ def listed():
         # the full training batch: dense fp32 gradient of the whole table
         dict(name="embed_grad_batch", op="embed_grad", n=16384, vocab=VOCAB, hidden=HIDDEN, dtype="fp32", scale=1.0,
              accumulate=False),
-        # one micro-batch of gradient accumulation: bf16 activations' gradient added into the fp32 main gradient
-        dict(name="embed_grad_accumulate", op="embed_grad", n=4096, vocab=VOCAB, hidden=HIDDEN, dtype="bf16",
-             scale=32.0, accumulate=True),
+        # scoring one sampled token against the crossbar lm_head's fp32 logits: one row, all latency
+        dict(name="logps_one_token", op="logps", n=1, vocab=VOCAB, seqs=1, dtype="fp32", temperature=1.0),
+        # scoring a batch of answers under the reference model, at the sampling temperature
+        dict(name="logps_batch", op="logps", n=2048, vocab=VOCAB, seqs=8, dtype="bf16", temperature=0.7),
         # toy policy step of a small test model: a few launches' worth of latency
         dict(name="policy_small", op="policy", n=96, vocab=512, seqs=2, dtype="fp32", kl_coef=0.0,
              reduction="token", temperature=1.0),
         # a policy-gradient micro-batch on the crossbar lm_head's fp32 logits, sequence-wise mean, KL to a reference
         dict(name="policy_fp32", op="policy", n=2047, vocab=VOCAB, seqs=8, dtype="fp32", kl_coef=0.05,
              reduction="sequence", temperature=1.0),
-        # a larger one with bf16 logits sampled at a temperature
-        dict(name="policy_bf16", op="policy", n=4096, vocab=VOCAB, seqs=16, dtype="bf16", kl_coef=0.05,
-             reduction="token", temperature=0.7),
         # four preference pairs of ragged answers, odd vocabulary: rows start on every alignment
         dict(name="preference_odd", op="preference", n=1501, vocab=32003, seqs=8, dtype="bf16", smoothing=0.1,
              temperature=1.0),
@@ -73,7 +72,7 @@ def _log_int(rng, lo, hi):
 
 
 def draw(rng):
-    op = rng.choice(["lookup", "embed_grad", "policy", "preference", "clip"])
+    op = rng.choice(["lookup", "embed_grad", "logps", "policy", "preference", "clip"])
     dtype = rng.choice(sorted(DTYPES))
     if op in ("lookup", "embed_grad"):
         vocab, hidden = _log_int(rng, 128, VOCAB), _log_int(rng, 64, 4096)
@@ -85,16 +84,16 @@ def draw(rng):
         if op == "embed_grad":
             case["accumulate"] = rng.random() < 0.4
         return case
-    if op in ("policy", "preference"):
+    if op in ("logps", "policy", "preference"):
         vocab = _log_int(rng, 128, VOCAB)
         if rng.random() < 0.5:
             vocab = max(128, vocab // 64 * 64)
-        seqs = 2 * _log_int(rng, 1, 16)
+        seqs = 1 if op == "logps" else 2 * _log_int(rng, 1, 16)
         n = min(_log_int(rng, seqs, 16384), max(seqs, 2047 * VOCAB // vocab))
         case = dict(op=op, n=n, vocab=vocab, seqs=seqs, dtype=dtype, temperature=rng.choice([1.0, 1.0, 0.7]))
         if op == "policy":
             case.update(kl_coef=rng.choice([0.0, 0.05]), reduction=rng.choice(["token", "sequence"]))
-        else:
+        elif op == "preference":
             case.update(smoothing=rng.choice([0.0, 0.1]))
         return case
     return dict(op="clip", layout="random", tensors=_log_int(rng, 1, 400), elements=_log_int(rng, 1000, 600_000_000),
@@ -167,7 +166,7 @@ def prepare(case, seed):
         if case["accumulate"]:
             st["out"] = torch.randn(vocab, hidden, generator=g, device=DEVICE) * 0.01
         return st
-    if case["op"] in ("policy", "preference"):
+    if case["op"] in ("logps", "policy", "preference"):
         n, vocab, temp = case["n"], case["vocab"], case["temperature"]
         cu, seq, place, length = _sequences(case, g)
         targets = torch.randint(0, vocab, (n,), generator=g, device=DEVICE)
@@ -175,8 +174,11 @@ def prepare(case, seed):
         logits = torch.randn(n, vocab, generator=g, device=DEVICE, dtype=dt) * 2.5
         front = 3.1 + math.log(vocab) - 1.0 + 1.5 * torch.randn(n, 1, generator=g, device=DEVICE)
         logits.scatter_(1, targets[:, None], front.to(dt))
-        lp = _row_logps(logits, targets, temp)
-        targets = torch.where(place * 4 < length, IGNORE, targets)          # the first quarter is the prompt
+        lp = None if case["op"] == "logps" else _row_logps(logits, targets, temp)
+        if n > 1:
+            targets = torch.where(place * 4 < length, IGNORE, targets)      # the first quarter is the prompt
+        if case["op"] == "logps":
+            return dict(case=case, logits=logits, targets=targets)
         ref = (lp + 0.2 * torch.randn(n, generator=g, device=DEVICE)).float()
         st = dict(case=case, logits=logits, targets=targets, ref=ref, cu=cu)
         if case["op"] == "policy":
@@ -212,19 +214,19 @@ def _plain_rows(st):
     e = torch.exp(x - m)
     s = e.sum(1, keepdim=True)
     lp = (x.gather(1, t) - m - torch.log(s))[:, 0]
-    return torch.where(valid, lp, 0.0), valid, e.div_(s), t
+    return torch.where(valid, lp, 0.0), valid, e, s, t
 
 
-def _plain_logit_grad(st, p, t, coef):
-    """coef_r (1{j = t_r} - p[r, j]) / T, rounded once."""
+def _plain_logit_grad(st, e, s, t, coef):
+    """coef_r (1{j = t_r} - e[r, j] / s_r) / T, rounded once."""
     coef = (coef / st["case"]["temperature"])[:, None]
-    g = p.mul_(-coef)
+    g = e.div_(s).mul_(-coef)
     return g.scatter_add_(1, t, coef).to(st["logits"].dtype)
 
 
 def _plain_policy(st):
     c = st["case"]
-    lp, valid, p, t = _plain_rows(st)
+    lp, valid, e, s, t = _plain_rows(st)
     row = torch.arange(c["n"], device=lp.device)
     seq = torch.searchsorted(st["cu"][1:], row, right=True)
     v = valid.float()
@@ -242,12 +244,12 @@ def _plain_policy(st):
     loss = (w * (torch.where(valid, -torch.minimum(free, held) + c["kl_coef"] * kl, 0.0))).sum()
     coef = torch.where(valid, w * (torch.where(clipped, 0.0, -free) + c["kl_coef"] * (1.0 - torch.exp(d))), 0.0)
     return {"loss": loss, "logps": lp, "kl": (w * torch.where(valid, kl, 0.0)).sum(),
-            "clip_fraction": (w * clipped).sum(), "grad": _plain_logit_grad(st, p, t, coef)}
+            "clip_fraction": (w * clipped).sum(), "grad": _plain_logit_grad(st, e, s, t, coef)}
 
 
 def _plain_preference(st):
     c = st["case"]
-    lp, valid, p, t = _plain_rows(st)
+    lp, valid, e, s, t = _plain_rows(st)
     row = torch.arange(c["n"], device=lp.device)
     seq = torch.searchsorted(st["cu"][1:], row, right=True)
     pairs = c["seqs"] // 2
@@ -261,7 +263,7 @@ def _plain_preference(st):
     side = torch.cat([slope, -slope]) * (0.1 / pairs)
     coef = torch.where(valid, side[seq], 0.0)
     return {"loss": loss, "chosen_rewards": chosen, "rejected_rewards": rejected, "logps": lp,
-            "grad": _plain_logit_grad(st, p, t, coef)}
+            "grad": _plain_logit_grad(st, e, s, t, coef)}
 
 
 def _plain(st):
@@ -273,6 +275,8 @@ def _plain(st):
         if c["accumulate"]:
             return st["out"].index_add_(0, st["ids"], g)
         return torch.zeros(c["vocab"], c["hidden"], device=g.device).index_add_(0, st["ids"], g).to(st["grad"].dtype)
+    if c["op"] == "logps":
+        return _plain_rows(st)[0]
     if c["op"] == "policy":
         return _plain_policy(st)
     if c["op"] == "preference":
@@ -293,6 +297,8 @@ def run(state):
     if c["op"] == "embed_grad":
         return NN_layers.embedding_scaled_grad(st["ids"], st["grad"], c["vocab"], c["scale"], out=st["out"],
                                                accumulate=c["accumulate"])
+    if c["op"] == "logps":
+        return tuning.token_logprobs(st["logits"], st["targets"], temperature=c["temperature"])
     if c["op"] == "policy":
         r, grad = tuning.policy_loss_grad(st["logits"], st["targets"], st["old"], st["adv"], st["ref"],
                                           cu_seqlens=st["cu"], clip_low=0.2, clip_high=0.28, kl_coef=c["kl_coef"],
@@ -317,9 +323,11 @@ def work(case):
         n, h = case["n"], case["hidden"]
         rows = 8 * h * _expected_rows(n, case["vocab"]) if case["accumulate"] else size * h * case["vocab"]
         return {"bytes": size * n * h + rows + 8 * n, "flops": 2 * n * h}
-    if case["op"] in ("policy", "preference"):
+    if case["op"] in ("logps", "policy", "preference"):
         n, v = case["n"], case["vocab"]
-        return {"bytes": 2 * size * n * v + 24 * n, "flops": 8 * n * v}
+        read = 0.75 * n if n > 1 else n                 # a prompt row's logits are not needed, its gradient is zero
+        written = 0 if case["op"] == "logps" else n
+        return {"bytes": size * v * (read + written) + 24 * n, "flops": 5 * read * v + 3 * written * v}
     return {"bytes": 2 * size * case["elements"], "flops": 3 * case["elements"]}
 
 
@@ -351,10 +359,12 @@ def exact(case, seed):
         return {"norm": torch.tensor(norm, dtype=f64), "clipped": flat}
     # the two losses: row quantities first, then sums over sequences on the host
     n, temp = case["n"], case["temperature"]
-    cu, targets = st["cu"].tolist(), st["targets"]
+    targets = st["targets"]
     keep = targets != IGNORE
     lp = torch.where(keep, _row_logps(st["logits"], targets, temp), 0.0)
-    slope = torch.zeros(n, dtype=f64, device=DEVICE)
+    if case["op"] == "logps":
+        return lp
+    slope, cu = torch.zeros(n, dtype=f64, device=DEVICE), st["cu"].tolist()
     spans = [(a, b, int(keep[a:b].sum())) for a, b in zip(cu[:-1], cu[1:])]
     ref = st["ref"].to(f64)
     out = {"logps": lp}
