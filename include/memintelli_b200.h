@@ -270,6 +270,102 @@ int mib_row_logsumexp(const float* logits, int64_t rows, int64_t cols, int64_t l
                       int64_t target_offset, float* row_max, float* row_sumexp, float* target_logit,
                       cudaStream_t stream);
 
+/* -------------------------------------------------------------------------------------------------
+ * Language-model tuning operators (outside the reference's CIM path, no reference counterpart): what a
+ * hardware-aware tuning step needs around the crossbar layers.  Element types are MIB_F32, MIB_BF16 and
+ * MIB_F16; arithmetic and sums are fp32 (or double where a sum is long), rounded once to the output type.
+ * Index lists are int32, or int64 where the *_i64 flag is set.  Workspaces are device memory, 256-byte
+ * aligned, sized by the *_workspace calls, and hold nothing between calls.
+ * ------------------------------------------------------------------------------------------------- */
+#define MIB_F32 0
+#define MIB_BF16 1
+#define MIB_F16 2
+
+/* out[i] = scale * table[ids[i]] for i < n; table (vocab, hidden) with rows ld_table apart, out (n, hidden)
+ * dense, both of type dtype.  An id outside [0, vocab) gives a row of NaN. */
+int mib_embedding_lookup(const void* ids, int32_t ids_i64, int64_t n, const void* table, int32_t dtype, int64_t vocab,
+                         int64_t hidden, int64_t ld_table, float scale, void* out, cudaStream_t stream);
+
+/* Gradient of the lookup: out[v] = scale * sum over i with ids[i] = v of grad[i], in ascending i (the same bits on
+ * every call); rows without a token become zero.  With accumulate the sums are added to `out` and other rows stay
+ * untouched.  Tokens equal to padding_idx (-1: none) and ids outside the table add nothing.  grad (n, hidden) with
+ * rows ld_grad apart; out (vocab, hidden), rows ld_out apart, of grad's type or MIB_F32. */
+int mib_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t hidden, int64_t* bytes_out);
+int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* grad, int32_t grad_dtype,
+                       int64_t ld_grad, int64_t vocab, int64_t hidden, float scale, int64_t padding_idx, void* out,
+                       int32_t out_dtype, int64_t ld_out, int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                       cudaStream_t stream);
+
+/* A (rows, cols) block of logits with a target column per row.  layout addresses rows as in mib_out_layout, with
+ * col_stride 1.  Rows whose target is ignore_index take no part: their logits are not read.  A target outside
+ * [0, cols) other than ignore_index makes its row's log-probability NaN.  Sequences (for entries that use them):
+ * sequence s holds rows [cu_seqlens[s], cu_seqlens[s + 1]) of a non-decreasing list of sequences + 1 offsets, or,
+ * with cu_seqlens NULL, rows_per_sequence rows each; rows outside every sequence take no part in a loss. */
+typedef struct mib_token_rows {
+  const void* logits;
+  const void* targets;
+  const void* cu_seqlens;
+  int64_t rows, cols;
+  mib_out_layout layout;
+  int64_t ignore_index;
+  int64_t sequences, rows_per_sequence;
+  double temperature;      /* log-probabilities are those of logits / temperature */
+  int32_t dtype, targets_i64, cu_i64, reserved;
+} mib_token_rows;
+
+/* Workspace of the three entries below (sequences 0 where there are none). */
+int mib_token_loss_workspace(int64_t rows, int64_t cols, int64_t sequences, int64_t* bytes_out);
+
+/* logps[r] = log softmax(logits[r] / temperature)[targets[r]], 0 where the target is ignore_index.  `stats`, when
+ * non-NULL (16 bytes per row, 16-byte aligned), keeps what the gradient needs of each row. */
+int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, void* workspace, int64_t workspace_bytes,
+                    cudaStream_t stream);
+
+/* Gradient of sum_r grad_logps[r] logps[r] over the same logits, in their type; `grad` may be the logits themselves. */
+int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float* grad_logps, void* grad,
+                         const mib_out_layout* grad_layout, cudaStream_t stream);
+
+/* Clipped policy loss.  Per token, ratio = exp(lp - old), d = ref - lp:
+ *   l = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1),
+ * loss = sum of w l with w = 1 / tokens (reduction 0), 1 / (sequences that have tokens) / (tokens of the sequence)
+ * (reduction 1) or 1 (reduction 2).  advantages has one entry per row, or per sequence (adv_per_sequence).
+ * ref_logps may be NULL when kl_coef is 0.  loss_kl_clip receives the loss, the weighted KL term without its
+ * coefficient and the weighted fraction of clipped tokens; logps the log-probabilities.  `grad`, when non-NULL,
+ * receives the gradient of the loss over the logits, in their type; it may be the logits themselves. */
+typedef struct mib_policy_spec {
+  double clip_low, clip_high, kl_coef;
+  int32_t reduction, adv_per_sequence;
+} mib_policy_spec;
+int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const float* old_logps,
+                    const float* advantages, const float* ref_logps, float* loss_kl_clip, float* logps, void* grad,
+                    const mib_out_layout* grad_layout, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
+/* Paired preference loss: pair i is sequence i (chosen) against sequence i + sequences / 2 (rejected).
+ *   D = sum over the sequence's tokens of lp - ref (their mean with `average`; ref_logps NULL counts as 0),
+ *   h = beta (D_chosen - D_rejected) - margin,
+ *   kind 0: -(1 - e) log sigmoid(h) - e log sigmoid(-h);  1: max(0, 1 - h);  2: (h - 1/2)^2;  loss = mean over pairs.
+ * chosen_rewards / rejected_rewards (sequences / 2 each) receive beta D.  `grad` as in mib_policy_loss. */
+typedef struct mib_preference_spec {
+  double beta, label_smoothing, margin;
+  int32_t kind, average;
+} mib_preference_spec;
+int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec, const float* ref_logps, float* loss,
+                        float* chosen_rewards, float* rejected_rewards, float* logps, void* grad,
+                        const mib_out_layout* grad_layout, void* workspace, int64_t workspace_bytes,
+                        cudaStream_t stream);
+
+/* x[i] *= *factor over n dense elements; a factor of exactly 1 leaves the buffer untouched. */
+int mib_scale_by(void* x, int32_t dtype, int64_t n, const float* factor, cudaStream_t stream);
+
+/* Global norm of `count` dense tensors (host arrays of device addresses, sizes and types) and, when `out` is
+ * non-NULL, out[i] = in[i] * min(1, max_norm / (norm + eps)); out[i] may be in[i].  norm_type is 1, 2 or 0 for
+ * infinity.  *norm (device) receives the norm before clipping; a NaN or infinity among the gradients shows there and,
+ * as the formula has it, in the clipped gradients. */
+int mib_clip_grad_norm_workspace(int32_t count, int64_t* bytes_out);
+int mib_clip_grad_norm(const void* const* in, void* const* out, const int64_t* numel, const int32_t* in_dtype,
+                       const int32_t* out_dtype, int32_t count, int32_t norm_type, float max_norm, float eps,
+                       float* norm, void* workspace, int64_t workspace_bytes, cudaStream_t stream);
+
 /* Reads and clears the device-side error flag of the current device (synchronises it).
  * Returns MIB_OK, or MIB_ERR_TIMEOUT when a kernel gave up a bounded wait. */
 int mib_device_status(void);

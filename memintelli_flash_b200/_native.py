@@ -49,6 +49,26 @@ class KGeom(ctypes.Structure):
     _fields_ = [("k", c_i64), ("kp", c_i64), ("p", c_i32), ("pp", c_i32), ("kt", c_i64)]
 
 
+# element types of the language-model tuning operators
+F32, BF16, F16 = 0, 1, 2
+
+
+class TokenRows(ctypes.Structure):
+    _fields_ = [("logits", c_vp), ("targets", c_vp), ("cu_seqlens", c_vp), ("rows", c_i64), ("cols", c_i64),
+                ("layout", OutLayout), ("ignore_index", c_i64), ("sequences", c_i64), ("rows_per_sequence", c_i64),
+                ("temperature", c_f64), ("dtype", c_i32), ("targets_i64", c_i32), ("cu_i64", c_i32),
+                ("reserved", c_i32)]
+
+
+class PolicySpec(ctypes.Structure):
+    _fields_ = [("clip_low", c_f64), ("clip_high", c_f64), ("kl_coef", c_f64), ("reduction", c_i32),
+                ("adv_per_sequence", c_i32)]
+
+
+class PreferenceSpec(ctypes.Structure):
+    _fields_ = [("beta", c_f64), ("label_smoothing", c_f64), ("margin", c_f64), ("kind", c_i32), ("average", c_i32)]
+
+
 _P = ctypes.POINTER
 _SIGS = {
     "mib_slice_input": [c_vp, c_i64, c_i64, c_i64, c_i64, c_i64, _P(SliceSpec), _P(KGeom), c_i32, c_i32,
@@ -77,6 +97,20 @@ _SIGS = {
     "mib_mvm_static_scratch": [c_vp, c_vp, c_i64, _P(SliceSpec), c_vp, c_vp, c_i64, _P(SliceSpec), _P(KGeom),
                                _P(DeviceSpec), c_i32, c_vp, c_i32, c_vp, _P(OutLayout), c_vp, c_vp],
     "mib_row_logsumexp": [c_vp, c_i64, c_i64, c_i64, c_vp, c_i64, c_vp, c_vp, c_vp, c_vp],
+    "mib_embedding_lookup": [c_vp, c_i32, c_i64, c_vp, c_i32, c_i64, c_i64, c_i64, c_f32, c_vp, c_vp],
+    "mib_embedding_grad_workspace": [c_i64, c_i64, c_i64, _P(c_i64)],
+    "mib_embedding_grad": [c_vp, c_i32, c_i64, c_vp, c_i32, c_i64, c_i64, c_i64, c_f32, c_i64, c_vp, c_i32, c_i64,
+                           c_i32, c_vp, c_i64, c_vp],
+    "mib_token_loss_workspace": [c_i64, c_i64, c_i64, _P(c_i64)],
+    "mib_token_logps": [_P(TokenRows), c_vp, c_vp, c_vp, c_i64, c_vp],
+    "mib_token_logps_grad": [_P(TokenRows), c_vp, c_vp, c_vp, _P(OutLayout), c_vp],
+    "mib_policy_loss": [_P(TokenRows), _P(PolicySpec), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, _P(OutLayout), c_vp,
+                        c_i64, c_vp],
+    "mib_preference_loss": [_P(TokenRows), _P(PreferenceSpec), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, _P(OutLayout),
+                            c_vp, c_i64, c_vp],
+    "mib_scale_by": [c_vp, c_i32, c_i64, c_vp, c_vp],
+    "mib_clip_grad_norm_workspace": [c_i32, _P(c_i64)],
+    "mib_clip_grad_norm": [c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_f32, c_f32, c_vp, c_vp, c_i64, c_vp],
     "mib_device_status": [],
     "mib_test_inject_wait_expiry": [c_i64],
 }

@@ -1,0 +1,360 @@
+// C ABI of the language-model tuning operators (declared in include/memintelli_b200.h): argument checks, workspace
+// layout and launches.  Included after memintelli_b200.cu's own entries (it uses their error helpers).
+
+namespace {
+
+bool known_dtype(int32_t d) { return d == MIB_F32 || d == MIB_BF16 || d == MIB_F16; }
+size_t dtype_size(int32_t d) { return d == MIB_F32 ? 4 : 2; }
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+
+// Calls fn with a value of the element type.
+template <typename F>
+cudaError_t with_dtype(int32_t d, F fn) {
+  if (d == MIB_F32) return fn(float());
+  if (d == MIB_BF16) return fn(__nv_bfloat16());
+  return fn(__half());
+}
+
+constexpr int64_t kMaxRows = int64_t(1) << 31;
+
+mib::RowMap row_map(const mib_out_layout& l) { return mib::RowMap{l.rows_per_group, l.group_stride, l.row_stride}; }
+
+int check_rows_layout(const mib_out_layout* l, int64_t rows, int64_t cols, const char* what) {
+  if (!l) return fail(MIB_ERR_PARAM, std::string(what) + " layout is NULL");
+  if (l->rows_per_group < 1 || l->col_stride != 1) return fail(MIB_ERR_SHAPE, std::string(what) + " needs unit column stride and rows in groups");
+  if (rows > 1 && l->rows_per_group > 1 && l->row_stride < cols)
+    return fail(MIB_ERR_SHAPE, std::string(what) + " rows overlap");
+  return MIB_OK;
+}
+
+int check_token_rows(const mib_token_rows* t) {
+  if (!t || !t->logits || !t->targets) return fail(MIB_ERR_PARAM, "NULL logits or targets");
+  if (!known_dtype(t->dtype)) return fail(MIB_ERR_UNSUPPORTED, "logits must be fp32, bf16 or fp16");
+  if (t->rows < 1 || t->cols < 1) return fail(MIB_ERR_SHAPE, "logits must be non-empty");
+  if (t->rows >= kMaxRows / 1024 || t->cols >= kMaxRows) return fail(MIB_ERR_SHAPE, "too many rows or columns");
+  if (!(t->temperature > 0.0) || !(t->temperature < 1e30)) return fail(MIB_ERR_PARAM, "temperature must be positive");
+  if (reinterpret_cast<uintptr_t>(t->logits) % dtype_size(t->dtype)) return fail(MIB_ERR_PARAM, "misaligned logits");
+  return check_rows_layout(&t->layout, t->rows, t->cols, "logits");
+}
+
+int check_sequences(const mib_token_rows* t) {
+  if (t->sequences < 0 || t->sequences >= kMaxRows / 2) return fail(MIB_ERR_SHAPE, "invalid number of sequences");
+  if (t->sequences > 0 && !t->cu_seqlens && t->rows_per_sequence < 1)
+    return fail(MIB_ERR_PARAM, "sequences need their row offsets or a common length");
+  return MIB_OK;
+}
+
+// Workspace of a loss: statistics of every (row, part), row coefficients, per-block sums, counters.
+struct TokenSpace {
+  int splits;
+  int64_t part, row, counts, seq_w, sums, done, bytes;
+};
+TokenSpace token_space(int64_t rows, int64_t cols, int64_t sequences) {
+  TokenSpace s;
+  s.splits = mib::row_splits(rows, cols);
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  s.part = take(rows * s.splits * static_cast<int64_t>(sizeof(mib::RowStat)));
+  s.row = take(rows * static_cast<int64_t>(sizeof(float4)));
+  s.counts = take(mib::kCountBlocks * 4);
+  s.seq_w = take(sequences * 4);
+  const int64_t blocks = (rows + 255) / 256 * 3;
+  s.sums = take((blocks > sequences ? blocks : sequences) * 8);
+  s.done = take(4);
+  s.bytes = at;
+  return s;
+}
+
+mib::TokenArgs token_args(const mib_token_rows* t, const TokenSpace& s, char* ws, float* logps, bool grad) {
+  mib::TokenArgs a{};
+  a.logits = t->logits;
+  a.map = row_map(t->layout);
+  a.rows = t->rows;
+  a.cols = t->cols;
+  a.targets = mib::IntList{t->targets, t->targets_i64};
+  a.ignore_index = t->ignore_index;
+  a.k = static_cast<float>(1.4426950408889634 / t->temperature);
+  a.inv_temp = 1.0 / t->temperature;
+  a.splits = s.splits;
+  a.part = reinterpret_cast<const mib::RowStat*>(ws + s.part);
+  a.logps = logps;
+  a.row = grad ? reinterpret_cast<float4*>(ws + s.row) : nullptr;
+  return a;
+}
+
+mib::SeqList seq_list(const mib_token_rows* t) {
+  return mib::SeqList{mib::IntList{t->cu_seqlens, t->cu_i64}, t->sequences, t->cu_seqlens ? 0 : t->rows_per_sequence};
+}
+
+int check_space(void* ws, int64_t have, int64_t need) {
+  if (!ws || have < need) return fail(MIB_ERR_PARAM, "workspace is missing or too small");
+  if (reinterpret_cast<uintptr_t>(ws) % 256) return fail(MIB_ERR_PARAM, "workspace must be 256-byte aligned");
+  return MIB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int mib_embedding_lookup(const void* ids, int32_t ids_i64, int64_t n, const void* table, int32_t dtype, int64_t vocab,
+                         int64_t hidden, int64_t ld_table, float scale, void* out, cudaStream_t stream) {
+  if (!ids || !table || !out) return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (!known_dtype(dtype)) return fail(MIB_ERR_UNSUPPORTED, "the table must be fp32, bf16 or fp16");
+  if (n < 1 || vocab < 1 || hidden < 1 || ld_table < hidden) return fail(MIB_ERR_SHAPE, "invalid embedding shape");
+  if (n >= kMaxRows || hidden > (1 << 24)) return fail(MIB_ERR_SHAPE, "too many tokens or columns");
+  cudaError_t e = with_dtype(dtype, [&](auto v) {
+    return mib::lookup_t<decltype(v)>(mib::IntList{ids, ids_i64}, n, table, vocab, hidden, ld_table, scale, out, stream);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "embedding_lookup launch");
+  return MIB_OK;
+}
+
+int mib_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t hidden, int64_t* bytes_out) {
+  if (!bytes_out) return fail(MIB_ERR_PARAM, "NULL argument");
+  if (n < 1 || vocab < 1 || hidden < 1) return fail(MIB_ERR_SHAPE, "invalid embedding shape");
+  *bytes_out = align256(static_cast<int64_t>(mib::embed_plan(n, vocab).bytes));
+  return MIB_OK;
+}
+
+int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* grad, int32_t grad_dtype,
+                       int64_t ld_grad, int64_t vocab, int64_t hidden, float scale, int64_t padding_idx, void* out,
+                       int32_t out_dtype, int64_t ld_out, int32_t accumulate, void* workspace, int64_t workspace_bytes,
+                       cudaStream_t stream) {
+  if (!ids || !grad || !out) return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (!known_dtype(grad_dtype) || (out_dtype != grad_dtype && out_dtype != MIB_F32))
+    return fail(MIB_ERR_UNSUPPORTED, "gradients are fp32, bf16 or fp16; the table's gradient has that type or fp32");
+  if (n < 1 || vocab < 1 || hidden < 1 || ld_grad < hidden || ld_out < hidden)
+    return fail(MIB_ERR_SHAPE, "invalid embedding shape");
+  if (n >= kMaxRows || vocab >= kMaxRows || hidden > (1 << 24)) return fail(MIB_ERR_SHAPE, "too many tokens, rows or columns");
+  if (int r = check_space(workspace, workspace_bytes, static_cast<int64_t>(mib::embed_plan(n, vocab).bytes))) return r;
+  mib::EmbedGradArgs a{};
+  a.n = n;
+  a.vocab = vocab;
+  a.hidden = hidden;
+  a.ld_grad = ld_grad;
+  a.ld_out = ld_out;
+  a.scale = scale;
+  a.accumulate = accumulate;
+  cudaError_t e = mib::sort_ids(mib::IntList{ids, ids_i64}, n, vocab, padding_idx, workspace, a, stream);
+  if (e == cudaSuccess)
+    e = with_dtype(grad_dtype, [&](auto v) {
+      using G = decltype(v);
+      return out_dtype == MIB_F32 ? mib::embed_grad_t<G, float>(a, grad, out, stream)
+                                  : mib::embed_grad_t<G, G>(a, grad, out, stream);
+    });
+  if (e != cudaSuccess) return cuda_fail(e, "embedding_grad launch");
+  return MIB_OK;
+}
+
+int mib_token_loss_workspace(int64_t rows, int64_t cols, int64_t sequences, int64_t* bytes_out) {
+  if (!bytes_out) return fail(MIB_ERR_PARAM, "NULL argument");
+  if (rows < 1 || cols < 1 || sequences < 0) return fail(MIB_ERR_SHAPE, "invalid logit block");
+  *bytes_out = token_space(rows, cols, sequences).bytes;
+  return MIB_OK;
+}
+
+int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, void* workspace, int64_t workspace_bytes,
+                    cudaStream_t stream) {
+  if (int r = check_token_rows(t)) return r;
+  if (!logps || reinterpret_cast<uintptr_t>(stats) % 16) return fail(MIB_ERR_PARAM, "NULL buffer");
+  const TokenSpace s = token_space(t->rows, t->cols, 0);
+  if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
+  char* ws = static_cast<char*>(workspace);
+  mib::TokenArgs a = token_args(t, s, ws, logps, false);
+  a.row = static_cast<float4*>(stats);
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
+    return mib::token_logps_t<decltype(v)>(a, reinterpret_cast<mib::RowStat*>(ws + s.part), stream);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "token_logps launch");
+  return MIB_OK;
+}
+
+int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float* grad_logps, void* grad,
+                         const mib_out_layout* grad_layout, cudaStream_t stream) {
+  if (int r = check_token_rows(t)) return r;
+  if (!stats || !grad_logps || !grad || reinterpret_cast<uintptr_t>(stats) % 16)
+    return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
+  if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+  mib::TokenArgs a = token_args(t, TokenSpace{}, nullptr, nullptr, false);
+  a.row = static_cast<float4*>(const_cast<void*>(stats));
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
+    return mib::logit_grad_t<decltype(v)>(a, grad_logps, grad, row_map(*grad_layout), stream);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "token_logps_grad launch");
+  return MIB_OK;
+}
+
+int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const float* old_logps,
+                    const float* advantages, const float* ref_logps, float* loss_kl_clip, float* logps, void* grad,
+                    const mib_out_layout* grad_layout, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  if (int r = check_token_rows(t)) return r;
+  if (int r = check_sequences(t)) return r;
+  if (!spec || !old_logps || !advantages || !loss_kl_clip || !logps) return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (!(spec->clip_low >= 0.0) || !(spec->clip_low <= 1.0) || !(spec->clip_high >= 0.0))
+    return fail(MIB_ERR_PARAM, "clip bounds must be non-negative, the lower one at most 1");
+  if (!(spec->kl_coef >= 0.0)) return fail(MIB_ERR_PARAM, "kl_coef must be non-negative");
+  if (spec->kl_coef > 0.0 && !ref_logps) return fail(MIB_ERR_PARAM, "the KL term needs reference log-probabilities");
+  if (spec->reduction < 0 || spec->reduction > 2) return fail(MIB_ERR_PARAM, "unknown reduction");
+  if ((spec->reduction == 1 || spec->adv_per_sequence) && t->sequences < 1)
+    return fail(MIB_ERR_PARAM, "a sequence mean or advantages per sequence need the sequences");
+  if (grad)
+    if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+  const TokenSpace s = token_space(t->rows, t->cols, t->sequences);
+  if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
+  char* ws = static_cast<char*>(workspace);
+  mib::PolicyArgs a{};
+  a.t = token_args(t, s, ws, logps, grad != nullptr);
+  a.seq = seq_list(t);
+  a.old_logps = old_logps;
+  a.advantages = advantages;
+  a.ref_logps = ref_logps;
+  a.adv_per_seq = spec->adv_per_sequence;
+  a.reduction = spec->reduction;
+  a.lo = static_cast<float>(1.0 - spec->clip_low);
+  a.hi = static_cast<float>(1.0 + spec->clip_high);
+  a.kl_coef = static_cast<float>(spec->kl_coef);
+  const int64_t want = spec->reduction == 1 ? (t->sequences + 7) / 8 : (t->rows + 255) / 256;
+  a.count_blocks = static_cast<int32_t>(want < mib::kCountBlocks ? want : mib::kCountBlocks);
+  a.counts = reinterpret_cast<int32_t*>(ws + s.counts);
+  a.seq_w = reinterpret_cast<float*>(ws + s.seq_w);
+  a.done = reinterpret_cast<uint32_t*>(ws + s.done);
+  a.sums = reinterpret_cast<double*>(ws + s.sums);
+  a.out = loss_kl_clip;
+  const mib::RowMap gmap = grad ? row_map(*grad_layout) : mib::RowMap{1, 0, 0};
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
+    return mib::policy_loss_t<decltype(v)>(a, reinterpret_cast<mib::RowStat*>(ws + s.part), grad, gmap, stream);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "policy_loss launch");
+  return MIB_OK;
+}
+
+int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec, const float* ref_logps, float* loss,
+                        float* chosen_rewards, float* rejected_rewards, float* logps, void* grad,
+                        const mib_out_layout* grad_layout, void* workspace, int64_t workspace_bytes,
+                        cudaStream_t stream) {
+  if (int r = check_token_rows(t)) return r;
+  if (int r = check_sequences(t)) return r;
+  if (!spec || !loss || !chosen_rewards || !rejected_rewards || !logps) return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (t->sequences < 2 || t->sequences % 2) return fail(MIB_ERR_SHAPE, "preference pairs need an even number of sequences");
+  if (spec->kind < 0 || spec->kind > 2) return fail(MIB_ERR_PARAM, "unknown preference loss");
+  if (!(spec->label_smoothing >= 0.0) || !(spec->label_smoothing <= 0.5) || (spec->kind != 0 && spec->label_smoothing != 0.0))
+    return fail(MIB_ERR_PARAM, "label smoothing must be in [0, 0.5], and 0 except for the sigmoid loss");
+  if (!(spec->beta > 0.0) || !(spec->beta < 1e30) || !(std::fabs(spec->margin) < 1e30))
+    return fail(MIB_ERR_PARAM, "beta must be positive and the margin finite");
+  if (grad)
+    if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+  const TokenSpace s = token_space(t->rows, t->cols, t->sequences);
+  if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
+  char* ws = static_cast<char*>(workspace);
+  mib::PreferenceArgs a{};
+  a.t = token_args(t, s, ws, logps, grad != nullptr);
+  a.seq = seq_list(t);
+  a.ref_logps = ref_logps;
+  a.kind = spec->kind;
+  a.average = spec->average;
+  a.beta = spec->beta;
+  a.smoothing = spec->label_smoothing;
+  a.margin = spec->margin;
+  a.done = reinterpret_cast<uint32_t*>(ws + s.done);
+  a.sums = reinterpret_cast<double*>(ws + s.sums);
+  a.chosen = chosen_rewards;
+  a.rejected = rejected_rewards;
+  a.out = loss;
+  const mib::RowMap gmap = grad ? row_map(*grad_layout) : mib::RowMap{1, 0, 0};
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
+    return mib::preference_loss_t<decltype(v)>(a, reinterpret_cast<mib::RowStat*>(ws + s.part), grad, gmap, stream);
+  });
+  if (e != cudaSuccess) return cuda_fail(e, "preference_loss launch");
+  return MIB_OK;
+}
+
+int mib_scale_by(void* x, int32_t dtype, int64_t n, const float* factor, cudaStream_t stream) {
+  if (!x || !factor) return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (!known_dtype(dtype)) return fail(MIB_ERR_UNSUPPORTED, "the buffer must be fp32, bf16 or fp16");
+  if (n < 1) return fail(MIB_ERR_SHAPE, "empty buffer");
+  cudaError_t e = with_dtype(dtype, [&](auto v) { return mib::scale_by_t<decltype(v)>(x, n, factor, stream); });
+  if (e != cudaSuccess) return cuda_fail(e, "scale_by launch");
+  return MIB_OK;
+}
+
+int mib_clip_grad_norm_workspace(int32_t count, int64_t* bytes_out) {
+  if (!bytes_out) return fail(MIB_ERR_PARAM, "NULL argument");
+  if (count < 0) return fail(MIB_ERR_SHAPE, "negative tensor count");
+  const int64_t launches = (static_cast<int64_t>(count) + mib::kClipTensors - 1) / mib::kClipTensors;
+  *bytes_out = align256(launches * mib::kClipBlocks * 8) + 256;
+  return MIB_OK;
+}
+
+int mib_clip_grad_norm(const void* const* in, void* const* out, const int64_t* numel, const int32_t* in_dtype,
+                       const int32_t* out_dtype, int32_t count, int32_t norm_type, float max_norm, float eps,
+                       float* norm, void* workspace, int64_t workspace_bytes, cudaStream_t stream) {
+  if (!norm || count < 0 || (count > 0 && (!in || !numel || !in_dtype || (out && !out_dtype))))
+    return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (norm_type < 0 || norm_type > 2) return fail(MIB_ERR_UNSUPPORTED, "norm_type must be 1, 2 or infinity");
+  if (out && (!(max_norm >= 0.0f) || !(eps >= 0.0f))) return fail(MIB_ERR_PARAM, "max_norm must be non-negative");
+  bool in_place = out != nullptr;
+  for (int32_t i = 0; i < count; ++i) {
+    if (numel[i] < 0 || numel[i] > (int64_t(1) << 40)) return fail(MIB_ERR_SHAPE, "invalid tensor size");
+    if (!known_dtype(in_dtype[i]) || (out && !known_dtype(out_dtype[i])))
+      return fail(MIB_ERR_UNSUPPORTED, "gradients must be fp32, bf16 or fp16");
+    if (numel[i] > 0 && (!in[i] || (out && !out[i]))) return fail(MIB_ERR_PARAM, "NULL tensor");
+    if (out && (out[i] != in[i] || out_dtype[i] != in_dtype[i])) in_place = false;
+  }
+  int64_t need = 0;
+  if (int r = mib_clip_grad_norm_workspace(count, &need)) return r;
+  if (int r = check_space(workspace, workspace_bytes, need)) return r;
+  mib::ClipState s{};
+  s.part = static_cast<double*>(workspace);
+  s.max_norm = max_norm;
+  s.eps = eps;
+  s.norm = norm;
+  s.coef = out ? reinterpret_cast<float*>(static_cast<char*>(workspace) + need - 256) : nullptr;
+
+  mib::ClipTable t;
+  for (int pass = 0; pass < (out ? 2 : 1); ++pass) {
+    int32_t i = 0;
+    while (i < count) {
+      t.count = 0;
+      t.first[0] = 0;
+      for (; i < count && t.count < mib::kClipTensors; ++i) {
+        if (numel[i] == 0) continue;
+        const int64_t chunks = (numel[i] + mib::kClipChunk - 1) / mib::kClipChunk;
+        if (t.first[t.count] + chunks > (int64_t(1) << 30)) {
+          if (t.count == 0) return fail(MIB_ERR_SHAPE, "tensor too large");
+          break;
+        }
+        const int k = t.count++;
+        t.in[k] = in[i];
+        t.out[k] = out ? out[i] : nullptr;
+        t.numel[k] = numel[i];
+        t.in_type[k] = static_cast<uint8_t>(in_dtype[i]);
+        t.out_type[k] = static_cast<uint8_t>(out ? out_dtype[i] : 0);
+        t.first[k + 1] = t.first[k] + static_cast<int32_t>(chunks);
+      }
+      if (t.count == 0) break;
+      cudaError_t e;
+      if (pass == 0) {
+        s.part_first = s.part_total;
+        s.part_total += static_cast<int32_t>(mib::clip_grid(t));
+        if (static_cast<int64_t>(s.part_total) * 8 > need - 256) return fail(MIB_ERR_SHAPE, "tensor list too large");
+        e = norm_type == 2 ? mib::clip_norm_p<2>(t, s, stream)
+                           : (norm_type == 1 ? mib::clip_norm_p<1>(t, s, stream) : mib::clip_norm_p<0>(t, s, stream));
+      } else {
+        e = mib::clip_scale(t, s.coef, in_place, stream);
+      }
+      if (e != cudaSuccess) return cuda_fail(e, "clip_grad_norm launch");
+    }
+    if (pass == 0) {
+      const cudaError_t e = norm_type == 2 ? mib::clip_finish_p<2>(s, stream)
+                                           : (norm_type == 1 ? mib::clip_finish_p<1>(s, stream) : mib::clip_finish_p<0>(s, stream));
+      if (e != cudaSuccess) return cuda_fail(e, "clip_grad_norm launch");
+    }
+  }
+  return MIB_OK;
+}
+
+}  // extern "C"

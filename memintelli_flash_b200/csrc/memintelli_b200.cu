@@ -18,6 +18,9 @@
 #include "mvm.cu"
 #include "attn_prep.cu"
 #include "row_lse.cu"
+#include "embedding.cu"
+#include "token_loss.cu"
+#include "grad_clip.cu"
 
 namespace {
 
@@ -949,3 +952,5 @@ extern "C" int mib_mvm_static_scratch(const void* a_planes, const float* a_scale
   return mib_mvm(a_planes, a_scale, m, x_spec, b_planes, b_scale, n, w_spec, kg, dev, operand_kind, adc_table,
                  adc_table_len, y, layout, bias, nullptr, scratch, need > 0 ? kStaticScratchFloats : 0, stream);
 }
+
+#include "lm_abi.cu"

@@ -1,0 +1,332 @@
+"""Losses on the logits of a language model, and token log-probabilities.
+
+``logits`` is (..., V), fp32, bf16 or fp16, on a CUDA device; ``targets`` holds the column of each row's token
+(shape ``logits.shape[:-1]``, int32 or int64), ``ignore_index`` where a row takes no part (prompt and padding): such a
+row's logits are not read, its log-probability is 0 and its gradient zero.  A target outside the vocabulary gives NaN.
+
+Sequences are the rows of a (B, T) batch of targets, or, with ``cu_seqlens`` (S + 1 non-decreasing row offsets),
+ragged ones packed in one list of rows.
+
+``policy_loss`` and ``preference_loss`` are differentiable in ``logits`` (the gradient is computed with the loss, in
+the forward call).  ``policy_loss_grad`` and ``preference_loss_grad`` return the loss and that gradient without
+autograd, into ``out`` if given: ``out=logits`` overwrites the logits and saves the gradient's memory.
+"""
+from __future__ import annotations
+
+from collections import namedtuple
+from functools import lru_cache
+
+import torch
+
+from .. import _native as N
+
+_DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
+_INTS = {torch.int32: 0, torch.int64: 1}
+_REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
+_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
+
+#: loss, per-token log-probabilities, weighted KL term (without its coefficient), weighted fraction of clipped tokens
+PolicyLoss = namedtuple("PolicyLoss", "loss logps kl clip_fraction")
+#: loss, beta times each pair's summed log ratio (chosen, rejected), per-token log-probabilities
+PreferenceLoss = namedtuple("PreferenceLoss", "loss chosen_rewards rejected_rewards logps")
+
+
+def _layout(t):
+    """Row addressing of a (..., V) tensor with unit column stride in at most two levels, or None."""
+    dims = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    merged = []
+    for n, s in reversed(dims):
+        if merged and s == merged[-1][0] * merged[-1][1]:
+            merged[-1] = (merged[-1][0] * n, merged[-1][1])
+        else:
+            merged.append((n, s))
+    if len(merged) > 2 or (t.shape[-1] != 1 and t.stride(-1) != 1):
+        return None
+    n, s = merged[0] if merged else (1, t.shape[-1])
+    if n > 1 and s < t.shape[-1]:
+        return None
+    return N.OutLayout(n, merged[1][1] if len(merged) == 2 else 0, s, 1)
+
+
+def _ints(t, what, device):
+    if t.dtype not in _INTS:
+        raise ValueError(f"{what} must be int32 or int64, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the logits on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _floats(t, what, shape, device):
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the logits on {device}")
+    return t.detach().to(torch.float32).contiguous()
+
+
+class _Rows:
+    """The checked rows of one call: the native description and the tensors it points into."""
+
+    def __init__(self, logits, targets, temperature, ignore_index, cu_seqlens=None):
+        if not logits.is_cuda:
+            raise ValueError("logits must be on a CUDA device")
+        if logits.dtype not in _DTYPES:
+            raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
+        if logits.dim() < 1 or logits.shape[-1] < 1:
+            raise ValueError("logits must be (..., V) with V >= 1")
+        if targets.shape != logits.shape[:-1]:
+            raise ValueError(f"targets has shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
+        if not 0.0 < temperature < 1e30:
+            raise ValueError("temperature must be positive")
+        dev = logits.device
+        logits = logits.detach()
+        layout = _layout(logits)
+        if layout is None:
+            logits = logits.contiguous()
+            layout = _layout(logits)
+        targets = _ints(targets, "targets", dev)
+        self.n = targets.numel()
+        if layout.rows_per_group < 1:            # no rows
+            layout.rows_per_group = 1
+        if cu_seqlens is not None:
+            if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+                raise ValueError("cu_seqlens must hold the S + 1 row offsets of S sequences")
+            cu_seqlens = _ints(cu_seqlens, "cu_seqlens", dev)
+            self.sequences, per = cu_seqlens.numel() - 1, 0
+        elif targets.dim() > 1:
+            per = targets.shape[-1]
+            self.sequences = self.n // per if per else 0
+        else:
+            self.sequences, per = 0, 0
+        self.logits, self.targets, self.cu, self.device = logits, targets, cu_seqlens, dev
+        self.spec = N.TokenRows(logits.data_ptr(), targets.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
+                                self.n, logits.shape[-1], layout, ignore_index, self.sequences, per, temperature,
+                                _DTYPES[logits.dtype], _INTS[targets.dtype],
+                                0 if cu_seqlens is None else _INTS[cu_seqlens.dtype], 0)
+
+    def workspace(self, sequences):
+        nbytes = _workspace_bytes(self.n, self.spec.cols, sequences)
+        return torch.empty(nbytes, dtype=torch.uint8, device=self.device), nbytes
+
+    def gradient(self, out):
+        """The gradient's tensor and row addressing."""
+        if out is None:
+            out = torch.empty(self.logits.shape, dtype=self.logits.dtype, device=self.device)
+        else:
+            if out.shape != self.logits.shape or out.dtype != self.logits.dtype or out.device != self.device:
+                raise ValueError("out must have the logits' shape, type and device")
+            if out.requires_grad and torch.is_grad_enabled():
+                raise ValueError("out must not require a gradient")
+        layout = _layout(out)
+        rows = 0 if layout is None else layout.rows_per_group
+        if layout is None or (self.n > rows and layout.group_stride < (rows - 1) * layout.row_stride + out.shape[-1]):
+            raise ValueError("out needs a unit column stride and rows that do not overlap")
+        a, b = self.logits, out
+        if a.data_ptr() == b.data_ptr():
+            if a.stride() != b.stride() and self.n > 1:
+                raise ValueError("out overlaps the logits without being the same rows")
+        elif a.numel() and _span(a)[0] < _span(b)[1] and _span(b)[0] < _span(a)[1]:
+            raise ValueError("out overlaps the logits without being the same rows")
+        if rows < 1:
+            layout.rows_per_group = 1
+        return out, layout
+
+
+def _span(t):
+    """First byte and one past the last byte that a tensor reaches."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(rows, cols, sequences):
+    n = N.c_i64(0)
+    N.call("mib_token_loss_workspace", rows, cols, sequences, n)
+    return n.value
+
+
+# ---- log-probabilities ---------------------------------------------------------------------------------
+class TokenLogprobsRunc(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, temperature, ignore_index):
+        rows = _Rows(logits, targets, temperature, ignore_index)
+        keep = ctx.needs_input_grad[0]
+        logps, stats = _token_logps(rows, keep)
+        if keep:
+            ctx.save_for_backward(logits, targets, stats)
+            ctx.args = (temperature, ignore_index)
+        return logps
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_logps):
+        logits, targets, stats = ctx.saved_tensors
+        rows = _Rows(logits, targets, *ctx.args)
+        grad, layout = rows.gradient(None)
+        if rows.n:
+            g = _floats(grad_logps, "the gradient", targets.shape, rows.device)
+            with N.device_guard(rows.device):
+                N.call("mib_token_logps_grad", rows.spec, N.ptr(stats), N.ptr(g), N.ptr(grad), layout,
+                       N.stream_ptr(rows.device))
+        return grad, None, None, None
+
+
+def _token_logps(rows, keep_stats):
+    logps = torch.empty(rows.targets.shape, dtype=torch.float32, device=rows.device)
+    stats = torch.empty(rows.n, 4, dtype=torch.float32, device=rows.device) if keep_stats else None
+    if rows.n:
+        ws, nbytes = rows.workspace(0)
+        with N.device_guard(rows.device):
+            N.call("mib_token_logps", rows.spec, N.ptr(logps), N.ptr(stats), N.ptr(ws), nbytes,
+                   N.stream_ptr(rows.device))
+    return logps, stats
+
+
+def token_logprobs(logits, targets, *, temperature=1.0, ignore_index=-100):
+    """log softmax(logits / temperature) at each row's target, fp32 (0 at ignored rows).  Differentiable in ``logits``."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobsRunc.apply(logits, targets, float(temperature), int(ignore_index))
+    return _token_logps(_Rows(logits, targets, float(temperature), int(ignore_index)), False)[0]
+
+
+# ---- policy loss ---------------------------------------------------------------------------------------
+def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, reduction,
+            temperature, ignore_index, want_grad, out):
+    rows = _Rows(logits, targets, float(temperature), int(ignore_index), cu_seqlens)
+    dev = rows.device
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
+    clip_high = clip_low if clip_high is None else clip_high
+    if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
+        raise ValueError("clip bounds must be non-negative and finite, the lower one at most 1")
+    if not 0.0 <= kl_coef < float("inf"):
+        raise ValueError("kl_coef must be non-negative")
+    if kl_coef > 0.0 and ref_logps is None:
+        raise ValueError("the KL term needs ref_logps")
+    if reduction == "sequence" and rows.sequences < 1 and rows.n:
+        raise ValueError("the sequence mean needs a (B, T) batch or cu_seqlens")
+    shape = targets.shape
+    old = _floats(old_logps, "old_logps", shape, dev)
+    per_token = advantages.shape == shape
+    if not per_token and (rows.sequences < 1 or advantages.numel() != rows.sequences):
+        raise ValueError(f"advantages has shape {tuple(advantages.shape)}, expected {tuple(shape)} or one per sequence "
+                         f"({rows.sequences})")
+    adv = _floats(advantages, "advantages", shape if per_token else advantages.shape, dev)
+    ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, dev)
+    grad, layout = rows.gradient(out) if want_grad else (None, None)
+    if rows.n == 0:
+        z = torch.zeros(3, dtype=torch.float32, device=dev)
+        return PolicyLoss(z[0], torch.zeros(shape, dtype=torch.float32, device=dev), z[1], z[2]), grad
+    logps = torch.empty(shape, dtype=torch.float32, device=dev)
+    res = torch.empty(3, dtype=torch.float32, device=dev)
+    ws, nbytes = rows.workspace(rows.sequences)
+    spec = N.PolicySpec(clip_low, clip_high, kl_coef, _REDUCTIONS[reduction], 0 if per_token else 1)
+    with N.device_guard(dev):
+        N.call("mib_policy_loss", rows.spec, spec, N.ptr(old), N.ptr(adv), N.ptr(ref), N.ptr(res), N.ptr(logps),
+               N.ptr(grad), layout, N.ptr(ws), nbytes, N.stream_ptr(dev))
+    loss, kl, clipped = res.unbind(0)
+    return PolicyLoss(loss, logps, kl, clipped), grad
+
+
+class _LossRunc(torch.autograd.Function):
+    """A loss whose gradient over the logits was computed with it: backward scales that gradient and hands it over."""
+
+    @staticmethod
+    def forward(ctx, logits, evaluate):
+        result, ctx.grad = evaluate(logits, ctx.needs_input_grad[0])
+        ctx.mark_non_differentiable(*result[1:])
+        return tuple(result)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss, *_):
+        grad, ctx.grad = ctx.grad, None
+        if grad is None:
+            raise RuntimeError("the loss's gradient was already handed over: a second backward pass needs a second "
+                               "forward pass")
+        if grad.numel():
+            factor = grad_loss.to(torch.float32).contiguous()
+            with N.device_guard(grad.device):
+                N.call("mib_scale_by", N.ptr(grad), _DTYPES[grad.dtype], grad.numel(), N.ptr(factor),
+                       N.stream_ptr(grad.device))
+        return grad, None
+
+
+def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=None, kl_coef=0.0,
+                cu_seqlens=None, reduction="token", temperature=1.0, ignore_index=-100):
+    """Clipped policy loss with a KL term to a reference policy; returns a ``PolicyLoss``.
+
+    Per token, with ``lp`` its log-probability, ``ratio = exp(lp - old_logps)`` and ``d = ref_logps - lp``:
+    ``-min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)``.  ``reduction``: "token"
+    (mean over the tokens that take part), "sequence" (mean over the sequences that have such tokens of their token
+    means) or "sum".  ``advantages``: one per token or one per sequence; ``clip_high`` defaults to ``clip_low``.
+    Without a token that takes part the loss is 0."""
+    def evaluate(x, want):
+        return _policy(x, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens,
+                       reduction, temperature, ignore_index, want, None)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return PolicyLoss(*_LossRunc.apply(logits, evaluate))
+    return evaluate(logits, False)[0]
+
+
+def policy_loss_grad(logits, targets, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=None,
+                     kl_coef=0.0, cu_seqlens=None, reduction="token", temperature=1.0, ignore_index=-100, out=None):
+    """``policy_loss`` and the gradient of its loss over the logits, in their type: ``(PolicyLoss, grad)``."""
+    return _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens,
+                   reduction, temperature, ignore_index, True, out)
+
+
+# ---- preference loss -----------------------------------------------------------------------------------
+def _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, margin, kind, average, temperature,
+                ignore_index, want_grad, out):
+    rows = _Rows(logits, targets, float(temperature), int(ignore_index), cu_seqlens)
+    dev = rows.device
+    if kind not in _KINDS:
+        raise ValueError(f"kind must be one of {sorted(_KINDS)}, got {kind!r}")
+    if not 0.0 <= label_smoothing <= 0.5 or (kind != "sigmoid" and label_smoothing):
+        raise ValueError("label_smoothing must be in [0, 0.5], and 0 except for the sigmoid loss")
+    if not 0.0 < beta < 1e30:
+        raise ValueError("beta must be positive")
+    if not abs(margin) < 1e30:
+        raise ValueError("margin must be finite")
+    if rows.sequences < 2 or rows.sequences % 2:
+        raise ValueError("preference pairs need an even number of sequences: the chosen ones, then the rejected ones "
+                         f"in the same order (got {rows.sequences})")
+    shape, pairs = targets.shape, rows.sequences // 2
+    ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, dev)
+    grad, layout = rows.gradient(out) if want_grad else (None, None)
+    logps = torch.empty(shape, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    chosen, rejected = (torch.empty(pairs, dtype=torch.float32, device=dev) for _ in range(2))
+    if rows.n == 0:
+        raise ValueError("preference pairs need rows")
+    ws, nbytes = rows.workspace(rows.sequences)
+    spec = N.PreferenceSpec(beta, label_smoothing, margin, _KINDS[kind], 1 if average else 0)
+    with N.device_guard(dev):
+        N.call("mib_preference_loss", rows.spec, spec, N.ptr(ref), N.ptr(loss), N.ptr(chosen), N.ptr(rejected),
+               N.ptr(logps), N.ptr(grad), layout, N.ptr(ws), nbytes, N.stream_ptr(dev))
+    return PreferenceLoss(loss, chosen, rejected, logps), grad
+
+
+def preference_loss(logits, targets, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0, margin=0.0,
+                    kind="sigmoid", average=False, temperature=1.0, ignore_index=-100):
+    """Preference loss over pairs of sequences; returns a ``PreferenceLoss``.
+
+    Of S sequences, sequence i (chosen) is paired with sequence i + S / 2 (rejected).  With ``D`` the sum over a
+    sequence's tokens of ``lp - ref_logps`` (their mean with ``average``; no ``ref_logps`` counts as 0) and
+    ``h = beta (D_chosen - D_rejected) - margin``, the mean over pairs of ``kind``: "sigmoid"
+    ``-(1 - e) log sigmoid(h) - e log sigmoid(-h)`` with ``e = label_smoothing``, "hinge" ``max(0, 1 - h)`` or
+    "squared" ``(h - 1/2)^2``.  A sequence without a token counts as D = 0."""
+    def evaluate(x, want):
+        return _preference(x, targets, ref_logps, cu_seqlens, beta, label_smoothing, margin, kind, average,
+                           temperature, ignore_index, want, None)
+    if logits.requires_grad and torch.is_grad_enabled():
+        return PreferenceLoss(*_LossRunc.apply(logits, evaluate))
+    return evaluate(logits, False)[0]
+
+
+def preference_loss_grad(logits, targets, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0,
+                         margin=0.0, kind="sigmoid", average=False, temperature=1.0, ignore_index=-100, out=None):
+    """``preference_loss`` and the gradient of its loss over the logits, in their type: ``(PreferenceLoss, grad)``."""
+    return _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, margin, kind, average,
+                       temperature, ignore_index, True, out)
