@@ -300,7 +300,8 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
  * col_stride 1.  Rows whose target is ignore_index take no part: their logits are not read.  A target outside
  * [0, cols) other than ignore_index makes its row's log-probability NaN.  Sequences (for entries that use them):
  * sequence s holds rows [cu_seqlens[s], cu_seqlens[s + 1]) of a non-decreasing list of sequences + 1 offsets, or,
- * with cu_seqlens NULL, rows_per_sequence rows each; rows outside every sequence take no part in a loss. */
+ * with cu_seqlens NULL, rows_per_sequence rows each; rows outside every sequence take no part in a loss (their logits
+ * are not read, their log-probability is written as 0). */
 typedef struct mib_token_rows {
   const void* logits;
   const void* targets;
@@ -313,17 +314,16 @@ typedef struct mib_token_rows {
   int32_t dtype, targets_i64, cu_i64, reserved;
 } mib_token_rows;
 
-/* Workspace of the three entries below (sequences 0 where there are none). */
-int mib_token_loss_workspace(int64_t rows, int64_t cols, int64_t sequences, int64_t* bytes_out);
-
 /* logps[r] = log softmax(logits[r] / temperature)[targets[r]], 0 where the target is ignore_index.  `stats`, when
  * non-NULL (16 bytes per row, 16-byte aligned), keeps what the gradient needs of each row. */
-int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, void* workspace, int64_t workspace_bytes,
-                    cudaStream_t stream);
+int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, cudaStream_t stream);
 
 /* Gradient of sum_r grad_logps[r] logps[r] over the same logits, in their type; `grad` may be the logits themselves. */
 int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float* grad_logps, void* grad,
                          const mib_out_layout* grad_layout, cudaStream_t stream);
+
+/* Workspace of the two losses below (sequences 0 where there are none). */
+int mib_token_loss_workspace(int64_t rows, int64_t cols, int64_t sequences, int64_t* bytes_out);
 
 /* Clipped policy loss.  Per token, ratio = exp(lp - old), d = ref - lp:
  *   l = -min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1),

@@ -102,7 +102,7 @@ _SIGS = {
     "mib_embedding_grad": [c_vp, c_i32, c_i64, c_vp, c_i32, c_i64, c_i64, c_i64, c_f32, c_i64, c_vp, c_i32, c_i64,
                            c_i32, c_vp, c_i64, c_vp],
     "mib_token_loss_workspace": [c_i64, c_i64, c_i64, _P(c_i64)],
-    "mib_token_logps": [_P(TokenRows), c_vp, c_vp, c_vp, c_i64, c_vp],
+    "mib_token_logps": [_P(TokenRows), c_vp, c_vp, c_vp],
     "mib_token_logps_grad": [_P(TokenRows), c_vp, c_vp, c_vp, _P(OutLayout), c_vp],
     "mib_policy_loss": [_P(TokenRows), _P(PolicySpec), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, _P(OutLayout), c_vp,
                         c_i64, c_vp],

@@ -44,32 +44,29 @@ int check_sequences(const mib_token_rows* t) {
   return MIB_OK;
 }
 
-// Workspace of a loss: statistics of every (row, part), row coefficients, per-block sums, counters.
+// Workspace of a loss: row coefficients and terms, per-pair sums, counters.
 struct TokenSpace {
-  int splits;
-  int64_t part, row, counts, seq_w, sums, done, bytes;
+  int64_t row, terms, counts, seq_w, sums, done, bytes;
 };
-TokenSpace token_space(int64_t rows, int64_t cols, int64_t sequences) {
+TokenSpace token_space(int64_t rows, int64_t sequences) {
   TokenSpace s;
-  s.splits = mib::row_splits(rows, cols);
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
     at += align256(bytes);
     return here;
   };
-  s.part = take(rows * s.splits * static_cast<int64_t>(sizeof(mib::RowStat)));
   s.row = take(rows * static_cast<int64_t>(sizeof(float4)));
+  s.terms = take(rows * static_cast<int64_t>(sizeof(float4)));
   s.counts = take(mib::kCountBlocks * 4);
   s.seq_w = take(sequences * 4);
-  const int64_t blocks = (rows + 255) / 256 * 3;
-  s.sums = take((blocks > sequences ? blocks : sequences) * 8);
+  s.sums = take(sequences * 8);
   s.done = take(4);
   s.bytes = at;
   return s;
 }
 
-mib::TokenArgs token_args(const mib_token_rows* t, const TokenSpace& s, char* ws, float* logps, bool grad) {
+mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
   mib::TokenArgs a{};
   a.logits = t->logits;
   a.map = row_map(t->layout);
@@ -79,10 +76,8 @@ mib::TokenArgs token_args(const mib_token_rows* t, const TokenSpace& s, char* ws
   a.ignore_index = t->ignore_index;
   a.k = static_cast<float>(1.4426950408889634 / t->temperature);
   a.inv_temp = 1.0 / t->temperature;
-  a.splits = s.splits;
-  a.part = reinterpret_cast<const mib::RowStat*>(ws + s.part);
   a.logps = logps;
-  a.row = grad ? reinterpret_cast<float4*>(ws + s.row) : nullptr;
+  a.row = static_cast<float4*>(row);
   return a;
 }
 
@@ -153,22 +148,16 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
 int mib_token_loss_workspace(int64_t rows, int64_t cols, int64_t sequences, int64_t* bytes_out) {
   if (!bytes_out) return fail(MIB_ERR_PARAM, "NULL argument");
   if (rows < 1 || cols < 1 || sequences < 0) return fail(MIB_ERR_SHAPE, "invalid logit block");
-  *bytes_out = token_space(rows, cols, sequences).bytes;
+  *bytes_out = token_space(rows, sequences).bytes;
   return MIB_OK;
 }
 
-int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, void* workspace, int64_t workspace_bytes,
-                    cudaStream_t stream) {
+int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, cudaStream_t stream) {
   if (int r = check_token_rows(t)) return r;
-  if (!logps || reinterpret_cast<uintptr_t>(stats) % 16) return fail(MIB_ERR_PARAM, "NULL buffer");
-  const TokenSpace s = token_space(t->rows, t->cols, 0);
-  if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
-  char* ws = static_cast<char*>(workspace);
-  mib::TokenArgs a = token_args(t, s, ws, logps, false);
-  a.row = static_cast<float4*>(stats);
-  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
-    return mib::token_logps_t<decltype(v)>(a, reinterpret_cast<mib::RowStat*>(ws + s.part), stream);
-  });
+  if (!logps || reinterpret_cast<uintptr_t>(stats) % 16) return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
+  mib::RowArgs a{};
+  a.t = token_args(t, logps, stats);
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::token_logps_t<decltype(v)>(a, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "token_logps launch");
   return MIB_OK;
 }
@@ -179,11 +168,12 @@ int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float
   if (!stats || !grad_logps || !grad || reinterpret_cast<uintptr_t>(stats) % 16)
     return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
   if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
-  mib::TokenArgs a = token_args(t, TokenSpace{}, nullptr, nullptr, false);
-  a.row = static_cast<float4*>(const_cast<void*>(stats));
-  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
-    return mib::logit_grad_t<decltype(v)>(a, grad_logps, grad, row_map(*grad_layout), stream);
-  });
+  mib::GradArgs g{};
+  g.t = token_args(t, nullptr, const_cast<void*>(stats));
+  g.slope = grad_logps;
+  g.grad = grad;
+  g.gmap = row_map(*grad_layout);
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::logit_grad_t<decltype(v)>(g, false, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "token_logps_grad launch");
   return MIB_OK;
 }
@@ -203,11 +193,11 @@ int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const 
     return fail(MIB_ERR_PARAM, "a sequence mean or advantages per sequence need the sequences");
   if (grad)
     if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
-  const TokenSpace s = token_space(t->rows, t->cols, t->sequences);
+  const TokenSpace s = token_space(t->rows, t->sequences);
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
-  mib::PolicyArgs a{};
-  a.t = token_args(t, s, ws, logps, grad != nullptr);
+  mib::RowArgs a{};
+  a.t = token_args(t, logps, nullptr);
   a.seq = seq_list(t);
   a.old_logps = old_logps;
   a.advantages = advantages;
@@ -217,17 +207,16 @@ int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const 
   a.lo = static_cast<float>(1.0 - spec->clip_low);
   a.hi = static_cast<float>(1.0 + spec->clip_high);
   a.kl_coef = static_cast<float>(spec->kl_coef);
-  const int64_t want = spec->reduction == 1 ? (t->sequences + 7) / 8 : (t->rows + 255) / 256;
+  const int64_t want = spec->reduction == 1 ? (t->sequences + 7) / 8 : (spec->reduction == 0 ? (t->rows + 255) / 256 : 1);
   a.count_blocks = static_cast<int32_t>(want < mib::kCountBlocks ? want : mib::kCountBlocks);
   a.counts = reinterpret_cast<int32_t*>(ws + s.counts);
   a.seq_w = reinterpret_cast<float*>(ws + s.seq_w);
   a.done = reinterpret_cast<uint32_t*>(ws + s.done);
-  a.sums = reinterpret_cast<double*>(ws + s.sums);
+  a.terms = reinterpret_cast<float4*>(ws + s.terms);
   a.out = loss_kl_clip;
-  const mib::RowMap gmap = grad ? row_map(*grad_layout) : mib::RowMap{1, 0, 0};
-  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
-    return mib::policy_loss_t<decltype(v)>(a, reinterpret_cast<mib::RowStat*>(ws + s.part), grad, gmap, stream);
-  });
+  a.grad = grad;
+  if (grad) a.gmap = row_map(*grad_layout);
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::policy_loss_t<decltype(v)>(a, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "policy_loss launch");
   return MIB_OK;
 }
@@ -247,27 +236,34 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
     return fail(MIB_ERR_PARAM, "beta must be positive and the margin finite");
   if (grad)
     if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
-  const TokenSpace s = token_space(t->rows, t->cols, t->sequences);
+  const TokenSpace s = token_space(t->rows, t->sequences);
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
+  mib::RowArgs rows{};
+  rows.t = token_args(t, logps, grad ? ws + s.row : nullptr);
+  rows.seq = seq_list(t);
+  rows.ref_logps = ref_logps;
+  rows.done = reinterpret_cast<uint32_t*>(ws + s.done);
+  rows.d = reinterpret_cast<double*>(ws + s.terms);
   mib::PreferenceArgs a{};
-  a.t = token_args(t, s, ws, logps, grad != nullptr);
-  a.seq = seq_list(t);
-  a.ref_logps = ref_logps;
+  a.t = rows.t;
+  a.seq = rows.seq;
+  a.d = rows.d;
   a.kind = spec->kind;
   a.average = spec->average;
   a.beta = spec->beta;
   a.smoothing = spec->label_smoothing;
   a.margin = spec->margin;
-  a.done = reinterpret_cast<uint32_t*>(ws + s.done);
+  a.done = rows.done;
   a.sums = reinterpret_cast<double*>(ws + s.sums);
   a.chosen = chosen_rewards;
   a.rejected = rejected_rewards;
   a.out = loss;
-  const mib::RowMap gmap = grad ? row_map(*grad_layout) : mib::RowMap{1, 0, 0};
-  cudaError_t e = with_dtype(t->dtype, [&](auto v) {
-    return mib::preference_loss_t<decltype(v)>(a, reinterpret_cast<mib::RowStat*>(ws + s.part), grad, gmap, stream);
-  });
+  mib::GradArgs g{};
+  g.t = rows.t;
+  g.grad = grad;
+  if (grad) g.gmap = row_map(*grad_layout);
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::preference_loss_t<decltype(v)>(rows, a, g, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "preference_loss launch");
   return MIB_OK;
 }

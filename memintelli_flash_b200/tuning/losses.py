@@ -175,10 +175,8 @@ def _token_logps(rows, keep_stats):
     logps = torch.empty(rows.targets.shape, dtype=torch.float32, device=rows.device)
     stats = torch.empty(rows.n, 4, dtype=torch.float32, device=rows.device) if keep_stats else None
     if rows.n:
-        ws, nbytes = rows.workspace(0)
         with N.device_guard(rows.device):
-            N.call("mib_token_logps", rows.spec, N.ptr(logps), N.ptr(stats), N.ptr(ws), nbytes,
-                   N.stream_ptr(rows.device))
+            N.call("mib_token_logps", rows.spec, N.ptr(logps), N.ptr(stats), N.stream_ptr(rows.device))
     return logps, stats
 
 

@@ -69,6 +69,7 @@ def policy(logits, targets, old, adv, ref, *, clip_low=0.2, clip_high=0.2, kl_co
     zero = torch.zeros((), dtype=torch.float64)
     pick = lambda v: torch.where(w > 0, v, zero)  # noqa: E731
     slope = pick(slope) * w
+    lp = torch.where(keep, lp, 0.0)
     return (pick(term) * w).sum(), lp, (pick(kl) * w).sum(), (clipped * w).sum(), logit_grad(p, targets, slope, temperature)
 
 
