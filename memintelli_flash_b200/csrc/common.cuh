@@ -13,9 +13,9 @@
 namespace mib {
 
 // ---------------------------------------------------------------------------
-// device error flag (set by kernels whose bounded waits expire)
+// device error flag (set by kernels whose bounded waits expire), one per translation unit
 // ---------------------------------------------------------------------------
-__device__ int g_device_error = 0;
+static __device__ int g_device_error = 0;
 
 // ~2 s at 1.9 GHz; no wait in a correct run comes near this.
 constexpr long long kWaitTimeoutCycles = 4000000000LL;

@@ -88,31 +88,186 @@ cudaError_t lookup_t(IntList ids, int64_t n, const void* table, int64_t vocab, i
   return cudaErrorMisalignedAddress;
 }
 
-// ---- stable radix sort of the ids --------------------------------------------------------------------
-constexpr int kSortTile = 2048, kSortThreads = 256, kDigits = 256;
+// ---- stable radix sort of the ids: up to 65536 tokens in one launch -------------------------------------
+// The blocks of one cluster (8, or a single block for up to 2048 tokens) hold all (id, position) pairs in registers
+// and sort them by up to 9 bits a pass, least significant first: ranks within a warp by match, counts of the warps
+// and blocks added through (distributed) shared memory.  151936 rows take two passes.  The grid's other blocks
+// meanwhile write the dense gradient's zeros, so the sort costs no time of its own next to a large table.
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kBins = 512, kSortCluster = 8;
+
+struct SortArgs {
+  IntList ids;
+  int64_t n, vocab, padding;
+  uint32_t *keys0, *keys1, *pos0, *pos1;  // scratch: even passes write 0, odd ones 1
+  int32_t passes, bits;
+  uint32_t* heads;             // [0]: number of split runs, zeroed here
+  // zeros of the dense gradient
+  void* zero;
+  int64_t zero_rows, zero_row_bytes, zero_pitch;
+};
 
 // Ids that add nothing (the padding row's, ids outside the table) take the key `vocab` and end up last.
 __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t vocab, int64_t padding) {
   return static_cast<uint32_t>(id < 0 || id >= vocab || id == padding ? vocab : id);
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_keys_kernel(IntList ids, int64_t n, int64_t vocab, int64_t padding,
+__device__ void write_zeros(const SortArgs& a, int64_t block, int64_t blocks) {
+  char* p = static_cast<char*>(a.zero);
+  const int64_t stride = blocks * blockDim.x, first = block * blockDim.x + threadIdx.x;
+  if (a.zero_pitch == a.zero_row_bytes && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+    const int64_t bytes = a.zero_rows * a.zero_row_bytes;
+    for (int64_t i = first; i < bytes / 16; i += stride) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = bytes / 16 * 16 + first * 2; i < bytes; i += stride * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
+  } else {
+    const int64_t per = a.zero_row_bytes / 2;
+    for (int64_t i = first; i < a.zero_rows * per; i += stride)
+      *reinterpret_cast<uint16_t*>(p + i / per * a.zero_pitch + i % per * 2) = 0;
+  }
+}
+
+template <int ITEMS>
+__global__ void __launch_bounds__(kSortThreads) sort_zero_kernel(SortArgs a) {
+  __shared__ uint16_t count[kSortWarps][kBins];
+  __shared__ uint16_t total[kSortCluster][kBins];
+  __shared__ uint32_t base[kBins];
+  __shared__ uint32_t warp_sum[kBins / 32];
+  pdl_release();
+  const uint32_t nranks = cluster_size(), rank = cluster_rank();
+  if (blockIdx.x >= nranks) {
+    write_zeros(a, blockIdx.x - nranks, gridDim.x - nranks);
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (rank == 0 && threadIdx.x == 0) a.heads[0] = 0;
+  if (nranks > 1) cluster_arrive();  // waited for in front of the first remote store
+  const int64_t first = (static_cast<int64_t>(rank) * kSortWarps + warp) * (32 * ITEMS) + lane;
+  for (int q = 0; q < a.passes; ++q) {
+    const int shift = q * a.bits;
+    const uint32_t* keys_in = (q & 1) ? a.keys0 : a.keys1;
+    const uint32_t* pos_in = (q & 1) ? a.pos0 : a.pos1;
+    uint32_t* keys_out = (q & 1) ? a.keys1 : a.keys0;
+    uint32_t* pos_out = (q & 1) ? a.pos1 : a.pos0;
+    const uint32_t mask = (1u << a.bits) - 1u;
+    uint32_t key[ITEMS], val[ITEMS], rnk[ITEMS];
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const int64_t i = first + u * 32;
+      key[u] = 0;
+      val[u] = static_cast<uint32_t>(i);
+      if (i < a.n) {
+        if (q == 0) {
+          key[u] = sort_key(a.ids[i], a.vocab, a.padding);
+        } else {
+          key[u] = __ldcg(keys_in + i);
+          val[u] = __ldcg(pos_in + i);
+        }
+      }
+    }
+    for (int d = lane; d < kBins; d += 32) count[warp][d] = 0;
+    __syncwarp();
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      const uint32_t d = first + u * 32 < a.n ? (key[u] >> shift) & mask : kBins;
+      const uint32_t peers = __match_any_sync(0xffffffffu, d);
+      const uint32_t seen = d < kBins ? count[warp][d] : 0;
+      rnk[u] = seen + __popc(peers & ((1u << lane) - 1u));
+      __syncwarp();
+      if (d < kBins && lane == 31 - __clz(peers)) count[warp][d] = static_cast<uint16_t>(seen + __popc(peers));
+      __syncwarp();
+    }
+    __syncthreads();
+    if (nranks > 1 && q == 0) cluster_wait();
+    if (threadIdx.x < kBins) {  // counts of the warps in front, and the block's own total to every block
+      const int d = threadIdx.x;
+      uint32_t s = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = count[w][d];
+        count[w][d] = static_cast<uint16_t>(s);
+        s += c;
+      }
+      if (nranks > 1) {
+        for (uint32_t b = 0; b < nranks; ++b) {
+          uint32_t to;
+          asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(&total[rank][d])), "r"(b));
+          asm volatile("st.shared::cluster.u16 [%0], %1;" ::"r"(to), "h"(static_cast<uint16_t>(s)) : "memory");
+        }
+      } else {
+        total[0][d] = static_cast<uint16_t>(s);
+      }
+    }
+    if (nranks > 1) {
+      cluster_arrive();
+      cluster_wait();
+    } else {
+      __syncthreads();
+    }
+    uint32_t all = 0, before = 0, scan = 0;
+    if (threadIdx.x < kBins) {
+      for (uint32_t b = 0; b < nranks; ++b) {
+        const uint32_t c = total[b][threadIdx.x];
+        if (b < rank) before += c;
+        all += c;
+      }
+      scan = all;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += y;
+      }
+      if (lane == 31) warp_sum[warp] = scan;
+    }
+    __syncthreads();
+    if (threadIdx.x < kBins) {
+      for (int w = 0; w < warp; ++w) scan += warp_sum[w];
+      base[threadIdx.x] = scan - all + before;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < ITEMS; ++u) {
+      if (first + u * 32 < a.n) {
+        const uint32_t d = (key[u] >> shift) & mask;
+        const uint32_t to = base[d] + count[warp][d] + rnk[u];
+        keys_out[to] = key[u];
+        pos_out[to] = val[u];
+      }
+    }
+    if (q + 1 < a.passes) {
+      if (nranks > 1) {
+        cluster_arrive();
+        cluster_wait();
+      } else {
+        __threadfence();
+        __syncthreads();
+      }
+    }
+  }
+}
+
+// ---- the same sort for more tokens: 8 bits a pass, three launches each ------------------------------------
+constexpr int kTile = 2048, kTileThreads = 256, kDigits = 256;
+
+
+__global__ void __launch_bounds__(kTileThreads) sort_keys_kernel(IntList ids, int64_t n, int64_t vocab, int64_t padding,
                                                                  uint32_t* __restrict__ keys,
-                                                                 uint32_t* __restrict__ pos) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * kSortThreads + threadIdx.x;
+                                                                 uint32_t* __restrict__ pos, uint32_t* heads) {
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * kTileThreads + threadIdx.x;
   if (i < n) {
     keys[i] = sort_key(ids[i], vocab, padding);
     pos[i] = static_cast<uint32_t>(i);
   }
+  if (i == 0) heads[0] = 0;
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_hist_kernel(const uint32_t* __restrict__ keys, int64_t n, int shift,
+__global__ void __launch_bounds__(1024) zero_kernel(SortArgs a) { write_zeros(a, blockIdx.x, gridDim.x); }
+
+__global__ void __launch_bounds__(kTileThreads) sort_hist_kernel(const uint32_t* __restrict__ keys, int64_t n, int shift,
                                                                  uint32_t* __restrict__ hist, int blocks) {
   __shared__ uint32_t h[kDigits];
   h[threadIdx.x] = 0;
   __syncthreads();
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kSortTile;
-  for (int i = threadIdx.x; i < kSortTile; i += kSortThreads)
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kTile;
+  for (int i = threadIdx.x; i < kTile; i += kTileThreads)
     if (lo + i < n) atomicAdd(&h[(keys[lo + i] >> shift) & (kDigits - 1)], 1u);
   __syncthreads();
   hist[static_cast<int64_t>(threadIdx.x) * blocks + blockIdx.x] = h[threadIdx.x];
@@ -146,17 +301,17 @@ __global__ void __launch_bounds__(1024) sort_scan_kernel(uint32_t* hist, int64_t
 }
 
 // Each warp ranks 256 consecutive keys of its tile, 32 at a time, in order.
-__global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const uint32_t* __restrict__ keys,
+__global__ void __launch_bounds__(kTileThreads) sort_scatter_kernel(const uint32_t* __restrict__ keys,
                                                                     const uint32_t* __restrict__ pos, int64_t n,
                                                                     int shift, const uint32_t* __restrict__ hist,
                                                                     int blocks, uint32_t* __restrict__ keys_out,
                                                                     uint32_t* __restrict__ pos_out) {
-  constexpr int kWarps = kSortThreads / 32, kPer = kSortTile / kWarps / 32;
+  constexpr int kWarps = kTileThreads / 32, kPer = kTile / kWarps / 32;
   __shared__ uint32_t start[kWarps][kDigits];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int d = lane; d < kDigits; d += 32) start[warp][d] = 0;
   __syncwarp();
-  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kSortTile + warp * (kSortTile / kWarps);
+  const int64_t lo = static_cast<int64_t>(blockIdx.x) * kTile + warp * (kTile / kWarps);
   uint32_t key[kPer], rank[kPer];
 #pragma unroll
   for (int u = 0; u < kPer; ++u) {
@@ -193,86 +348,295 @@ __global__ void __launch_bounds__(kSortThreads) sort_scatter_kernel(const uint32
 }
 
 // ---- gradient -----------------------------------------------------------------------------------------
+// The sorted positions are cut into chunks; a group of threads, one per column vector, walks its chunk's tokens in
+// order, eight rows in flight, and writes each run that lies inside the chunk.  A run that crosses chunk borders
+// leaves one partial sum per chunk (slot 0 of the chunks it enters, slot 1 of the one it starts in), and its first
+// chunk goes on the list of split runs, which the join kernel adds up, in order.  The cut depends on n alone, so the
+// bits are the same every time.
 struct EmbedGradArgs {
   const uint32_t *keys, *pos;  // sorted
   int64_t n, vocab, hidden, ld_grad, ld_out;
   float scale;
-  int32_t accumulate;
+  int32_t accumulate, chunk;
+  float* partial;              // [chunks][2][hidden]
+  uint32_t* heads;             // [0] number, [1 ...] first chunks of the split runs
+  const void* grad;
+  void* out;
 };
 
-// First sorted position whose key is >= v.
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* __restrict__ keys, int64_t n, uint32_t v) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (__ldg(keys + mid) < v) lo = mid + 1; else hi = mid;
+// V consecutive elements.
+template <typename T, int V>
+__device__ __forceinline__ void load_cols(const T* p, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else if constexpr (V == kVec16<T>) {
+    unpack16<T>(*reinterpret_cast<const uint4*>(p), v);
+  } else {  // fp32 in vectors of 16-bit elements' length
+    float a[4], b[4];
+    unpack16<float>(*reinterpret_cast<const uint4*>(p), a);
+    unpack16<float>(*(reinterpret_cast<const uint4*>(p) + 1), b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = a[e];
+      v[e + 4] = b[e];
+    }
   }
-  return lo;
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_cols(T* p, const float (&v)[V]) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (V == kVec16<T>) {
+    *reinterpret_cast<uint4*>(p) = pack16<T>(v);
+  } else {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+    *(reinterpret_cast<float4*>(p) + 1) = make_float4(v[4], v[5], v[6], v[7]);
+  }
 }
 
-// One warp per table row: the run is summed in token order, a column at a time per lane.
-template <typename G, typename O>
-__global__ void __launch_bounds__(256) embed_grad_kernel(EmbedGradArgs a, const G* __restrict__ grad, O* out) {
-  const int lane = threadIdx.x & 31;
-  const int64_t v = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (v >= a.vocab) return;
-  const int64_t lo = lower_bound(a.keys, a.n, static_cast<uint32_t>(v));
-  int64_t hi = lo;
-  while (hi < a.n && __ldg(a.keys + hi) == static_cast<uint32_t>(v)) ++hi;
-  O* o = out + v * a.ld_out;
-  if (lo == hi && a.accumulate) return;
-  for (int64_t c = lane; c < a.hidden; c += 32) {
+template <typename O, int V>
+__device__ __forceinline__ void write_run(const EmbedGradArgs& a, uint32_t row, int64_t col, float (&s)[V]) {
+  O* o = static_cast<O*>(a.out) + static_cast<int64_t>(row) * a.ld_out + col;
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] *= a.scale;
+  if (a.accumulate) {
+    float old[V];
+    load_cols<O, V>(o, old);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] += old[e];
+  }
+  store_cols<O, V>(o, s);
+}
+
+// V columns of a row as they are stored.
+template <typename G, int V>
+struct RawCols {
+  using type = uint4;
+  static __device__ __forceinline__ uint4 load(const G* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+  static __device__ __forceinline__ void add(const uint4& u, float (&s)[V]) {
+    float v[V];
+    unpack16<G>(u, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] += v[e];
+  }
+};
+template <typename G>
+struct RawCols<G, 1> {
+  using type = G;
+  static __device__ __forceinline__ G load(const G* p) { return __ldg(p); }
+  static __device__ __forceinline__ void add(G u, float (&s)[1]) { s[0] += to_f32(u); }
+};
+
+template <typename G, typename O, int V>
+__global__ void __launch_bounds__(256) embed_sum_kernel(EmbedGradArgs a) {
+  constexpr int U = 8;
+  pdl_release();
+  pdl_wait();
+  const int64_t col = (static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x) * V;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t begin = c * a.chunk, end = begin + a.chunk < a.n ? begin + a.chunk : a.n;
+  if (begin >= a.n || col >= a.hidden) return;
+  const uint32_t none = static_cast<uint32_t>(a.vocab);
+  const uint32_t in = begin > 0 ? __ldcg(a.keys + begin - 1) : none;  // the key in front of the chunk
+  const uint32_t out = end < a.n ? __ldcg(a.keys + end) : none;       // the one behind it
+  const G* grad = static_cast<const G*>(a.grad) + col;
+  uint32_t run = __ldcg(a.keys + begin);
+  bool entered = run == in;  // the run began in an earlier chunk
+  float s[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) s[e] = 0.0f;
+  for (int64_t i0 = begin; i0 < end && run != none; i0 += U) {
+    uint32_t key[U];
+    typename RawCols<G, V>::type v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) key[u] = i0 + u < end ? __ldcg(a.keys + i0 + u) : none;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (key[u] != none) v[u] = RawCols<G, V>::load(grad + static_cast<int64_t>(__ldcg(a.pos + i0 + u)) * a.ld_grad);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u >= end) break;
+      if (key[u] != run) {  // uniform over the chunk's threads
+        if (entered) store_cols<float, V>(a.partial + (2 * c) * a.hidden + col, s);
+        else write_run<O, V>(a, run, col, s);
+        entered = false;
+        run = key[u];
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] = 0.0f;
+        if (run == none) break;
+      }
+      RawCols<G, V>::add(v[u], s);
+    }
+  }
+  if (run == none) return;
+  if (entered) {
+    store_cols<float, V>(a.partial + (2 * c) * a.hidden + col, s);
+  } else if (run == out) {
+    store_cols<float, V>(a.partial + (2 * c + 1) * a.hidden + col, s);
+    if (blockIdx.y == 0 && threadIdx.x == 0) a.heads[1 + atomicAdd(a.heads, 1u)] = static_cast<uint32_t>(c);
+  } else {
+    write_run<O, V>(a, run, col, s);
+  }
+}
+
+// Adds up the split runs: 32 columns and 8 stretches of a run's chunks per block, the stretches' sums joined in order.
+template <typename O>
+__global__ void __launch_bounds__(256) embed_join_kernel(EmbedGradArgs a) {
+  __shared__ float part[8][33];
+  pdl_wait();
+  const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
+  const int64_t col = static_cast<int64_t>(blockIdx.y) * 32 + lane;
+  const uint32_t count = __ldcg(a.heads);
+  for (uint32_t h = blockIdx.x; h < count; h += gridDim.x) {
+    const int64_t c = __ldcg(a.heads + 1 + h);
+    const uint32_t run = __ldcg(a.keys + (c + 1) * a.chunk);
+    // the run's last chunk: the one that holds its last position
+    int64_t lo = (c + 1) * a.chunk, hi = a.n;  // keys[lo] == run; first position past the run in (lo, hi]
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (__ldcg(a.keys + mid) == run) lo = mid; else hi = mid;
+    }
+    const int64_t m = lo / a.chunk - c;  // chunks c + 1 .. c + m hold the rest in their slot 0
+    const int64_t per = (m + 7) / 8, first = g * per, last = first + per < m ? first + per : m;
     float s = 0.0f;
-    for (int64_t i = lo; i < hi; ++i) s += to_f32(grad[static_cast<int64_t>(__ldg(a.pos + i)) * a.ld_grad + c]);
-    s *= a.scale;
-    if (a.accumulate) s += to_f32(o[c]);
-    o[c] = from_f32<O>(s);
+    if (col < a.hidden) {
+      const float* p = a.partial + col;
+      if (g == 0) s = __ldcg(p + (2 * c + 1) * a.hidden);
+#pragma unroll 8
+      for (int64_t i = first; i < last; ++i) s += __ldcg(p + 2 * (c + 1 + i) * a.hidden);
+    }
+    part[g][lane] = s;
+    __syncthreads();
+    if (g == 0 && col < a.hidden) {
+      float t[1] = {part[0][lane]};
+      for (int w = 1; w < 8; ++w) t[0] += part[w][lane];
+      write_run<O, 1>(a, run, col, t);
+    }
+    __syncthreads();
   }
 }
 
 struct EmbedPlan {
-  int64_t n, blocks;
-  int passes;
-  size_t bytes;
+  int items, cluster, passes, bits;  // items 0: the multi-launch sort
+  int64_t blocks, chunk, chunks;
+  size_t keys, hist, heads, partial, bytes;
 };
-EmbedPlan embed_plan(int64_t n, int64_t vocab) {
-  EmbedPlan p;
-  p.n = n;
-  p.blocks = (n + kSortTile - 1) / kSortTile;
-  p.passes = 1;
-  while ((vocab >> (8 * p.passes)) > 0) ++p.passes;
-  p.bytes = static_cast<size_t>(16 * n) + static_cast<size_t>(p.blocks) * kDigits * 4;
+// Chunks of 8 to 64 tokens, about 512 of them.
+EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t hidden) {
+  EmbedPlan p{};
+  int width = 1;
+  while ((vocab >> width) > 0) ++width;  // keys are 0 .. vocab
+  p.blocks = (n + kTile - 1) / kTile;
+  if (n <= 65536) {
+    p.cluster = n <= 2 * kSortThreads ? 1 : kSortCluster;
+    const int64_t per = static_cast<int64_t>(p.cluster) * kSortThreads;
+    p.items = n <= per ? 1 : (n <= 2 * per ? 2 : (n <= 4 * per ? 4 : 8));
+    p.passes = (width + 8) / 9;
+    p.bits = (width + p.passes - 1) / p.passes;
+  } else {
+    p.passes = (width + 7) / 8;
+  }
+  p.chunk = 8;
+  while (p.chunk < 64 && n > p.chunk * 512) p.chunk *= 2;
+  p.chunks = (n + p.chunk - 1) / p.chunk;
+  auto take = [&](size_t bytes) {
+    const size_t at = p.bytes;
+    p.bytes += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  p.keys = take(16 * static_cast<size_t>(n));
+  p.hist = take(p.items ? 0 : static_cast<size_t>(p.blocks) * kDigits * 4);
+  p.heads = take(4 * static_cast<size_t>(p.chunks + 1));
+  p.partial = take(8 * static_cast<size_t>(p.chunks) * static_cast<size_t>(hidden));
   return p;
 }
 
-template <typename G, typename O>
-cudaError_t embed_grad_t(EmbedGradArgs a, const void* grad, void* out, cudaStream_t stream) {
-  embed_grad_kernel<G, O><<<static_cast<unsigned>((a.vocab + 7) / 8), 256, 0, stream>>>(
-      a, static_cast<const G*>(grad), static_cast<O*>(out));
+cudaError_t sort_tiles(const SortArgs& s, const EmbedPlan& p, uint32_t* hist, cudaStream_t stream) {
+  const unsigned blocks = static_cast<unsigned>(p.blocks);
+  const int b = static_cast<int>(p.blocks);
+  sort_keys_kernel<<<static_cast<unsigned>((s.n + kTileThreads - 1) / kTileThreads), kTileThreads, 0, stream>>>(
+      s.ids, s.n, s.vocab, s.padding, s.keys1, s.pos1, s.heads);
   count_launch();
+  for (int q = 0; q < p.passes; ++q) {
+    uint32_t *keys_in = s.keys1, *pos_in = s.pos1, *keys_out = s.keys0, *pos_out = s.pos0;
+    if (q & 1) {
+      std::swap(keys_in, keys_out);
+      std::swap(pos_in, pos_out);
+    }
+    sort_hist_kernel<<<blocks, kTileThreads, 0, stream>>>(keys_in, s.n, 8 * q, hist, b);
+    sort_scan_kernel<<<1, 1024, 0, stream>>>(hist, p.blocks * kDigits);
+    sort_scatter_kernel<<<blocks, kTileThreads, 0, stream>>>(keys_in, pos_in, s.n, 8 * q, hist, b, keys_out, pos_out);
+    count_launch(3);
+  }
+  if (s.zero_rows > 0) {
+    zero_kernel<<<148, 1024, 0, stream>>>(s);
+    count_launch();
+  }
   return cudaGetLastError();
 }
 
-cudaError_t sort_ids(IntList ids, int64_t n, int64_t vocab, int64_t padding, void* workspace, EmbedGradArgs& a,
-                     cudaStream_t stream) {
-  const EmbedPlan p = embed_plan(n, vocab);
-  uint32_t* k0 = static_cast<uint32_t*>(workspace);
-  uint32_t *p0 = k0 + n, *k1 = p0 + n, *p1 = k1 + n, *hist = p1 + n;
-  const unsigned blocks = static_cast<unsigned>(p.blocks);
-  sort_keys_kernel<<<static_cast<unsigned>((n + kSortThreads - 1) / kSortThreads), kSortThreads, 0, stream>>>(
-      ids, n, vocab, padding, k0, p0);
+template <typename G, typename O, int V>
+cudaError_t embed_sum_v(const EmbedGradArgs& a, const EmbedPlan& p, cudaStream_t stream) {
+  const int64_t cols = a.hidden / V;
+  int x = 32;
+  while (x < 256 && x < cols) x *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(x, 256 / x);
+  cfg.gridDim = dim3(static_cast<unsigned>((p.chunks + 256 / x - 1) / (256 / x)), static_cast<unsigned>((cols + x - 1) / x));
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
   count_launch();
-  for (int q = 0; q < p.passes; ++q) {
-    sort_hist_kernel<<<blocks, kSortThreads, 0, stream>>>(k0, n, 8 * q, hist, static_cast<int>(p.blocks));
-    sort_scan_kernel<<<1, 1024, 0, stream>>>(hist, p.blocks * kDigits);
-    sort_scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(k0, p0, n, 8 * q, hist, static_cast<int>(p.blocks), k1, p1);
-    count_launch(3);
-    std::swap(k0, k1);
-    std::swap(p0, p1);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, embed_sum_kernel<G, O, V>, a);
+  if (e != cudaSuccess || p.chunks == 1) return e;
+  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.chunks < 64 ? p.chunks : 64), static_cast<unsigned>((a.hidden + 31) / 32));
+  count_launch();
+  return cudaLaunchKernelEx(&cfg, embed_join_kernel<O>, a);
+}
+
+template <typename G, typename O>
+cudaError_t embed_grad_t(EmbedGradArgs a, SortArgs s, void* workspace, cudaStream_t stream) {
+  const EmbedPlan p = embed_plan(a.n, a.vocab, a.hidden);
+  char* ws = static_cast<char*>(workspace);
+  uint32_t* scratch = reinterpret_cast<uint32_t*>(ws + p.keys);
+  s.keys0 = scratch;
+  s.pos0 = scratch + a.n;
+  s.keys1 = scratch + 2 * a.n;
+  s.pos1 = scratch + 3 * a.n;
+  s.heads = a.heads = reinterpret_cast<uint32_t*>(ws + p.heads);
+  a.partial = reinterpret_cast<float*>(ws + p.partial);
+  a.chunk = static_cast<int32_t>(p.chunk);
+  s.passes = p.passes;
+  s.bits = p.bits;
+  a.keys = (p.passes & 1) ? s.keys0 : s.keys1;
+  a.pos = (p.passes & 1) ? s.pos0 : s.pos1;
+  s.zero = a.out;
+  s.zero_rows = a.accumulate ? 0 : a.vocab;
+  s.zero_row_bytes = a.hidden * static_cast<int64_t>(sizeof(O));
+  s.zero_pitch = a.ld_out * static_cast<int64_t>(sizeof(O));
+  cudaError_t e;
+  if (p.items == 0) {
+    e = sort_tiles(s, p, reinterpret_cast<uint32_t*>(ws + p.hist), stream);
+  } else {
+    // blocks that write zeros: 64 KB each, at most the SMs that the sort leaves
+    int64_t fill = (s.zero_rows * s.zero_row_bytes + 65535) / 65536;
+    if (fill > 136) fill = 136;
+    const int64_t blocks = p.cluster + (fill + p.cluster - 1) / p.cluster * p.cluster;
+    auto fn = p.items == 1 ? sort_zero_kernel<1>
+                           : (p.items == 2 ? sort_zero_kernel<2> : (p.items == 4 ? sort_zero_kernel<4> : sort_zero_kernel<8>));
+    e = launch_kernel(fn, blocks, kSortThreads, p.cluster, false, s, stream);
   }
-  a.keys = k0;
-  a.pos = p0;
-  return cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  constexpr int V = kVec16<G>;
+  const uint64_t bits = reinterpret_cast<uintptr_t>(a.grad) | reinterpret_cast<uintptr_t>(a.out) |
+                        static_cast<uint64_t>(a.ld_grad) * sizeof(G) | static_cast<uint64_t>(a.ld_out) * sizeof(O) |
+                        static_cast<uint64_t>(a.hidden) * sizeof(G);
+  if (bits % 16 == 0) return embed_sum_v<G, O, V>(a, p, stream);
+  return embed_sum_v<G, O, 1>(a, p, stream);
 }
 
 }  // namespace mib

@@ -131,6 +131,10 @@ cudaError_t row_lse(const float* x, int64_t rows, int64_t cols, int64_t ld, cons
                     int64_t target_offset, float* row_max, float* row_sumexp, float* target_logit,
                     cudaStream_t stream);
 void count_launch(int n = 1);
+// Keeps a message for mib_last_error and returns the code.
+int record_error(int code, const char* msg);
+// Reads and clears the device error flag of the tuning operators' module (lm_ops.cu).
+cudaError_t lm_take_device_error(int* code);
 size_t mvm_smem_bytes(const MvmArgs& a);
 cudaError_t launch_splitk_reduce(const float* partial, int splits, int64_t M, int64_t N, float* y,
                                  int64_t rows_per_group, int64_t group_stride, int64_t row_stride,

@@ -1,7 +1,18 @@
 // C ABI of the language-model tuning operators (declared in include/memintelli_b200.h): argument checks, workspace
-// layout and launches.  Included after memintelli_b200.cu's own entries (it uses their error helpers).
+// layout and launches.
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "kernels.cuh"
 
 namespace {
+
+int fail(int code, const char* msg) { return mib::record_error(code, msg); }
+int fail(int code, const std::string& msg) { return mib::record_error(code, msg.c_str()); }
+int cuda_fail(cudaError_t e, const char* what) {
+  return fail(MIB_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
 
 bool known_dtype(int32_t d) { return d == MIB_F32 || d == MIB_BF16 || d == MIB_F16; }
 size_t dtype_size(int32_t d) { return d == MIB_F32 ? 4 : 2; }
@@ -76,6 +87,7 @@ mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
   a.ignore_index = t->ignore_index;
   a.k = static_cast<float>(1.4426950408889634 / t->temperature);
   a.inv_temp = 1.0 / t->temperature;
+  a.inv_temp_k = static_cast<double>(a.k) * 0.6931471805599453;
   a.logps = logps;
   a.row = static_cast<float4*>(row);
   return a;
@@ -111,7 +123,7 @@ int mib_embedding_lookup(const void* ids, int32_t ids_i64, int64_t n, const void
 int mib_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t hidden, int64_t* bytes_out) {
   if (!bytes_out) return fail(MIB_ERR_PARAM, "NULL argument");
   if (n < 1 || vocab < 1 || hidden < 1) return fail(MIB_ERR_SHAPE, "invalid embedding shape");
-  *bytes_out = align256(static_cast<int64_t>(mib::embed_plan(n, vocab).bytes));
+  *bytes_out = align256(static_cast<int64_t>(mib::embed_plan(n, vocab, hidden).bytes));
   return MIB_OK;
 }
 
@@ -125,7 +137,7 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
   if (n < 1 || vocab < 1 || hidden < 1 || ld_grad < hidden || ld_out < hidden)
     return fail(MIB_ERR_SHAPE, "invalid embedding shape");
   if (n >= kMaxRows || vocab >= kMaxRows || hidden > (1 << 24)) return fail(MIB_ERR_SHAPE, "too many tokens, rows or columns");
-  if (int r = check_space(workspace, workspace_bytes, static_cast<int64_t>(mib::embed_plan(n, vocab).bytes))) return r;
+  if (int r = check_space(workspace, workspace_bytes, static_cast<int64_t>(mib::embed_plan(n, vocab, hidden).bytes))) return r;
   mib::EmbedGradArgs a{};
   a.n = n;
   a.vocab = vocab;
@@ -134,13 +146,18 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
   a.ld_out = ld_out;
   a.scale = scale;
   a.accumulate = accumulate;
-  cudaError_t e = mib::sort_ids(mib::IntList{ids, ids_i64}, n, vocab, padding_idx, workspace, a, stream);
-  if (e == cudaSuccess)
-    e = with_dtype(grad_dtype, [&](auto v) {
-      using G = decltype(v);
-      return out_dtype == MIB_F32 ? mib::embed_grad_t<G, float>(a, grad, out, stream)
-                                  : mib::embed_grad_t<G, G>(a, grad, out, stream);
-    });
+  a.grad = grad;
+  a.out = out;
+  mib::SortArgs s{};
+  s.ids = mib::IntList{ids, ids_i64};
+  s.n = n;
+  s.vocab = vocab;
+  s.padding = padding_idx;
+  cudaError_t e = with_dtype(grad_dtype, [&](auto v) {
+    using G = decltype(v);
+    return out_dtype == MIB_F32 ? mib::embed_grad_t<G, float>(a, s, workspace, stream)
+                                : mib::embed_grad_t<G, G>(a, s, workspace, stream);
+  });
   if (e != cudaSuccess) return cuda_fail(e, "embedding_grad launch");
   return MIB_OK;
 }

@@ -1,7 +1,7 @@
 // C ABI of the B200 CIM sliced matmul (declared in include/memintelli_b200.h).
 //
-// One translation unit: the kernel sources are included here so the device
-// error flag and the kernels share a module.  This layer validates arguments
+// The kernel sources are included here so the device error flag and the kernels share a
+// module (the language-model tuning operators are a second one, lm_ops.cu).  This layer validates arguments
 // with the reference's error semantics, derives the kernel parameter blocks,
 // encodes the TMA tensor maps and launches.  It never allocates memory.
 #include <cudaTypedefs.h>
@@ -18,9 +18,6 @@
 #include "mvm.cu"
 #include "attn_prep.cu"
 #include "row_lse.cu"
-#include "embedding.cu"
-#include "token_loss.cu"
-#include "grad_clip.cu"
 
 namespace {
 
@@ -38,6 +35,14 @@ int fail(int code, const std::string& msg) {
 int cuda_fail(cudaError_t e, const char* what) {
   return fail(MIB_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
+
+}  // namespace
+
+namespace mib {
+int record_error(int code, const char* msg) { return fail(code, msg); }
+}  // namespace mib
+
+namespace {
 
 struct SliceTab {
   int S = 0, bits = 0;
@@ -426,6 +431,12 @@ int mib_device_status(void) {
   if (v != 0) {
     const int zero = 0;
     cudaMemcpyToSymbol(mib::g_device_error, &zero, sizeof(int));
+  }
+  int w = 0;  // the tuning operators' flag
+  e = mib::lm_take_device_error(&w);
+  if (e != cudaSuccess) return cuda_fail(e, "read device error flag");
+  if (v == 0) v = w;
+  if (v != 0) {
     char buf[96];
     snprintf(buf, sizeof(buf), "a bounded device wait expired (site %d)", v);
     return fail(MIB_ERR_TIMEOUT, buf);
@@ -952,5 +963,3 @@ extern "C" int mib_mvm_static_scratch(const void* a_planes, const float* a_scale
   return mib_mvm(a_planes, a_scale, m, x_spec, b_planes, b_scale, n, w_spec, kg, dev, operand_kind, adc_table,
                  adc_table_len, y, layout, bias, nullptr, scratch, need > 0 ? kStaticScratchFloats : 0, stream);
 }
-
-#include "lm_abi.cu"

@@ -65,19 +65,71 @@ __device__ __forceinline__ float vec_max(const uint4& u, float m) {
   }
 }
 
-// sum of 2^((v - m) k) over a vector, as a tree.
-template <typename T>
-__device__ __forceinline__ float vec_sum(const uint4& u, float m, float k) {
-  float v[kVec16<T>];
+// The reference of a set of exponentials 2^((v - m) k).  The fast form is 2^(v k - mk) in one fused operation, with mk
+// the rounded m k; `corr` (a relative correction of the results, at most 4e-4 with a square of 2e-7) makes up for that
+// rounding.  Where m k is larger (rows of a type's lowest value, say) v - m comes first: equal values give exactly 1.
+struct ExpRef {
+  float m, mk, corr;
+  bool fast;
+  __device__ __forceinline__ void set(float max, float k) {
+    m = max;
+    mk = max * k;
+    corr = -0.6931472f * fmaf(max, k, -mk);
+    fast = fabsf(mk) < 8192.0f;
+    if (!fast) corr = 0.0f;
+  }
+};
+
+// The exponentials of a vector's elements (without the correction).
+template <typename T, bool FAST>
+__device__ __forceinline__ void vec_exp(const uint4& u, const ExpRef& r, float k, float (&v)[kVec16<T>]) {
   unpack16<T>(u, v);
 #pragma unroll
-  for (int e = 0; e < kVec16<T>; ++e) v[e] = ex2((v[e] - m) * k);
-#pragma unroll
-  for (int w = kVec16<T> / 2; w > 0; w >>= 1)
-#pragma unroll
-    for (int e = 0; e < w; ++e) v[e] += v[e + w];
-  return v[0];
+  for (int e = 0; e < kVec16<T>; ++e) v[e] = ex2(FAST ? fmaf(v[e], k, -r.mk) : (v[e] - r.m) * k);
 }
+
+// Their sum over N vectors, as a tree, corrected.
+template <typename T, bool FAST, int N>
+__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, float k) {
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float v[kVec16<T>];
+    vec_exp<T, FAST>(u[i], r, k, v);
+#pragma unroll
+    for (int w = kVec16<T> / 2; w > 0; w >>= 1)
+#pragma unroll
+      for (int e = 0; e < w; ++e) v[e] += v[e + w];
+    s += v[0];
+  }
+  return fmaf(s, r.corr, s);
+}
+template <typename T, int N>
+__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, float k) {
+  return r.fast ? vecs_sum<T, true>(u, r, k) : vecs_sum<T, false>(u, r, k);
+}
+
+// N vectors of logits to q times their exponentials, in the logits' type.
+template <typename T, bool FAST, int N>
+__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, float k, float q) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float v[kVec16<T>];
+    vec_exp<T, FAST>(u[i], r, k, v);
+#pragma unroll
+    for (int e = 0; e < kVec16<T>; ++e) v[e] *= q;
+    u[i] = pack16<T>(v);
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, float k, float q) {
+  if (r.fast) vecs_grad<T, true>(u, r, k, q);
+  else vecs_grad<T, false>(u, r, k, q);
+}
+
+// Mean relative error of ex2.approx over its argument's fractions, measured on a B200 (2^20 arguments in [-24, 0]).
+// A sum of many exponentials carries it; summed over a sequence's tokens it would outgrow the rounding errors.
+constexpr float kEx2Mean = -5.2e-8f;
 
 // log s for s in (0, 2^127]: exponent and mantissa apart, so that the error is that of the log of a number near 1
 // (3e-8) and not half an ulp of the result (5e-7 for a vocabulary's sum).  0 gives -inf, NaN and inf themselves.
@@ -94,15 +146,19 @@ struct TokenArgs {
   int64_t rows, cols;
   IntList targets;
   int64_t ignore_index;
-  float k;             // log2(e) / T
-  double inv_temp;
+  float k;             // log2(e) / T, rounded
+  double inv_temp;     // 1 / T
+  double inv_temp_k;   // k log(2): 1 / T as k has it, which the target's logit takes like the others
   float* logps;        // [rows]
   float4* row;         // [rows] {m, 1 / s, c, -}, or null
 };
 
 __device__ __forceinline__ double row_logp(const TokenArgs& a, RowStat st, float target_logit, int64_t t) {
   if (t < 0 || t >= a.cols) return static_cast<double>(NAN);
-  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp - log_sum(st.s);
+  // the largest logit's exponential is 1 exactly, the rest of the sum has the mean error
+  const float bias = kEx2Mean * (1.0f - __frcp_rn(fmaxf(st.s, 1.0f)));
+  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp_k - log_sum(st.s) +
+         static_cast<double>(bias);
 }
 
 // Sequence s holds rows [cu[s], cu[s + 1]); both ends are held to [0, rows] whatever the list says.
@@ -158,9 +214,6 @@ struct RowArgs {
 
 constexpr int kCountBlocks = 64;
 
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // Tokens that take part: all (token mean), or per sequence with the number of non-empty ones (sequence mean).
 __global__ void __launch_bounds__(256) policy_count_kernel(RowArgs a) {
   __shared__ int smem[8];
@@ -198,7 +251,7 @@ struct RowScalars {
   float target_logit, old, adv, ref, w;
 };
 
-enum RowMode : int { kLogps = 0, kPolicy = 1, kPreference = 2 };
+enum RowMode : int { kStats = 0, kPolicy = 1 };
 
 template <typename T, int MODE>
 __device__ __forceinline__ RowScalars load_scalars(const RowArgs& a, int64_t r, int64_t t) {
@@ -220,7 +273,7 @@ __device__ __forceinline__ RowScalars load_scalars(const RowArgs& a, int64_t r, 
       if (a.reduction == 1) o.w *= __ldcg(a.seq_w + s);
     }
   }
-  if constexpr (MODE == kPreference) o.ref = a.ref_logps ? a.ref_logps[r] : 0.0f;
+  if (MODE == kStats && a.ref_logps) o.ref = a.ref_logps[r];
   return o;
 }
 
@@ -250,18 +303,6 @@ __device__ __forceinline__ float4 policy_term(const RowArgs& a, const RowScalars
 }
 
 // ---- clusters: the blocks of a cluster share a row ---------------------------------------------------
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
-__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_store(RowStat* p, uint32_t rank, RowStat v) {
   uint32_t to;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
@@ -278,14 +319,44 @@ __device__ __forceinline__ RowStat warp_merge(RowStat t, float k) {
   return RowStat{m, s};
 }
 
+// The loss and its statistics from the rows' terms, by the block that arrived last.
+template <int WARPS>
+__device__ __forceinline__ void add_terms(const RowArgs& a) {
+  __shared__ double smem[WARPS];
+  __threadfence();
+  double x = 0.0, y = 0.0, z = 0.0;
+  for (int64_t i = threadIdx.x; i < a.t.rows; i += blockDim.x) {
+    const float4 f = __ldcg(a.terms + i);
+    x += f.x;
+    y += f.y;
+    z += f.z;
+  }
+  x = block_sum(x, smem);
+  y = block_sum(y, smem);
+  z = block_sum(z, smem);
+  if (threadIdx.x == 0) {
+    a.out[0] = static_cast<float>(x);
+    a.out[1] = static_cast<float>(y);
+    a.out[2] = static_cast<float>(z);
+  }
+}
+
+// A vector's elements one by one, to a place off its alignment.
+template <typename T>
+__device__ __forceinline__ void store_elements(const uint4& v, uint4* to) {
+  if (!to) return;
+  const T* x = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int e = 0; e < kVec16<T>; ++e) reinterpret_cast<T*>(to)[e] = x[e];
+}
+
 constexpr int kMaxCluster = 8;
 
 // One row per GROUP threads of a block (a warp: four rows per block), or per cluster of blocks of 512.  RESIDENT rows
 // are held in registers, NV 16-byte vectors a thread, from their one load to the gradient's store; longer rows are
 // read twice (the second time from L2, where a cluster's one row has stayed).
-//   kLogps:      lp (and m, 1 / s for a later gradient)
-//   kPolicy:     lp, the loss's terms, and, if asked for, the gradient
-//   kPreference: lp, lp - ref, and m, 1 / s
+//   kStats:   lp and, where asked for, m and 1 / s for a later gradient, and lp - ref
+//   kPolicy:  lp, the loss's terms, and, where asked for, the gradient
 template <typename T, int GROUP, int NV, bool RESIDENT, int MODE>
 __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 1) token_row_kernel(RowArgs a) {
   constexpr int kWarps = GROUP / 32, V = kVec16<T>;
@@ -298,10 +369,10 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
   const int64_t r = kBlock ? blockIdx.x / nranks : static_cast<int64_t>(blockIdx.x) * (128 / GROUP) + threadIdx.x / GROUP;
   const bool have = r < a.t.rows;
   if (kBlock && nranks > 1) cluster_arrive();
-  if (MODE == kPreference) pdl_release();
+  if (MODE == kStats) pdl_release();
 
   const int64_t t = have ? a.t.targets[r] : a.t.ignore_index;
-  const bool live = t != a.t.ignore_index && (MODE == kLogps || a.seq.covers(r));
+  const bool live = t != a.t.ignore_index && a.seq.covers(r);
   const T* p = static_cast<const T*>(a.t.logits) + (have ? a.t.map.at(r) : 0);
   const int cols = static_cast<int>(a.t.cols), head = static_cast<int>(peel(p, a.t.cols));
   const int nvec = (cols - head) / V;
@@ -316,6 +387,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
   uint4 v[NV];
   float edge = -INFINITY, coef = 0.0f;
   RowStat st{kLowest, 0.0f};
+  ExpRef ref;
   if (live) {
     const uint32_t none = neg_inf_word<T>();
     if (edge_at >= 0) edge = to_f32(p[edge_at]);
@@ -336,9 +408,8 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       for (int u = 0; u < NV; ++u) st.m = vec_max<T>(v[u], st.m);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) st.m = fmaxf(st.m, __shfl_xor_sync(0xffffffffu, st.m, o));
-      st.s = ex2((edge - st.m) * a.t.k);
-#pragma unroll
-      for (int u = 0; u < NV; ++u) st.s += vec_sum<T>(v[u], st.m, a.t.k);
+      ref.set(st.m, a.t.k);
+      st.s = vecs_sum<T>(v, ref, a.t.k) + ex2((edge - st.m) * a.t.k);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
     } else {
@@ -349,10 +420,8 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
           v[u] = i + u * GROUP < left ? load_stream(pv + i + u * GROUP) : make_uint4(none, none, none, none);
 #pragma unroll
         for (int u = 0; u < NV; ++u) m = vec_max<T>(v[u], m);
-        float s = 0.0f;
-#pragma unroll
-        for (int u = 0; u < NV; ++u) s += vec_sum<T>(v[u], m, a.t.k);
-        st.s = fmaf(st.s, ex2((st.m - m) * a.t.k), s);
+        ref.set(m, a.t.k);
+        st.s = fmaf(st.s, ex2((st.m - m) * a.t.k), vecs_sum<T>(v, ref, a.t.k));
         st.m = m;
       }
       const float m = fmaxf(edge, st.m);
@@ -383,8 +452,8 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
     if (rank == 0 && tid == 0) {
       a.t.logps[r] = static_cast<float>(lp);
       if constexpr (MODE == kPolicy) a.terms[r] = term;
-      if constexpr (MODE == kPreference) a.d[r] = lp - static_cast<double>(sc.ref);
-      if (MODE != kPolicy && a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / st.s, 0.0f, 0.0f);
+      if (MODE == kStats && a.d) a.d[r] = lp - static_cast<double>(sc.ref);
+      if (MODE == kStats && a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / st.s, 0.0f, 0.0f);
     }
   } else {
     if (kBlock && nranks > 1) cluster_wait();
@@ -392,11 +461,11 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
     if (have && rank == 0 && tid == 0) {
       a.t.logps[r] = 0.0f;
       if constexpr (MODE == kPolicy) a.terms[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if constexpr (MODE == kPreference) a.d[r] = 0.0;
-      if (MODE != kPolicy && a.t.row) a.t.row[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+      if (MODE == kStats && a.d) a.d[r] = 0.0;
+      if (MODE == kStats && a.t.row) a.t.row[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
     }
   }
-  if (MODE == kPreference && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
+  if (MODE == kStats && a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
 
   if constexpr (MODE == kPolicy) {
     // the block (of rank 0) whose rows' terms are the last to arrive adds them all, below
@@ -411,77 +480,398 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
     if (a.grad && have) {
       T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
       const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-      const float q = -coef / st.s;
+      ref.set(st.m, a.t.k);
+      const float q0 = -coef / st.s, q = fmaf(q0, ref.corr, q0);
       const bool zero = coef == 0.0f;  // zeros whatever the logits hold, NaN and infinities included
-      float at_t = 0.0f;
-      int target_at = -1;  // the target among this thread's vectors, in elements from its first
-      if (!zero && t >= 0 && t < cols) {
-        const float x = kBlock ? shared_scalars.target_logit : to_f32(p[t]);
-        at_t = fmaf(q, ex2((x - st.m) * a.t.k), coef);
-        target_at = static_cast<int>(t) - head - at * V;
-      }
+      const bool hit = t >= 0 && t < cols;
+      float target_logit = 0.0f;
+      if (hit) target_logit = kBlock ? shared_scalars.target_logit : to_f32(p[t]);
       if (!kBlock) __syncwarp();  // in place: the target's logit is read before it is overwritten
       uint4* gv = reinterpret_cast<uint4*>(g + head) + at;
-      auto put = [&](const uint4& raw, int i) {
-        float x[V];
+      auto store = [&](int i0) {
         if (zero) {
 #pragma unroll
-          for (int e = 0; e < V; ++e) x[e] = 0.0f;
+          for (int u = 0; u < NV; ++u) v[u] = make_uint4(0, 0, 0, 0);
         } else {
-          unpack16<T>(raw, x);
-#pragma unroll
-          for (int e = 0; e < V; ++e) x[e] = q * ex2((x[e] - st.m) * a.t.k);
-          if (static_cast<uint32_t>(target_at - i * V) < static_cast<uint32_t>(V)) {
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-              if (target_at - i * V == e) x[e] = at_t;
-          }
+          vecs_grad<T>(v, ref, a.t.k, q);
         }
         if (same) {
-          __stcs(gv + i, pack16<T>(x));
-        } else {
-          T* to = reinterpret_cast<T*>(gv) + static_cast<int64_t>(i) * V;
 #pragma unroll
-          for (int e = 0; e < V; ++e) to[e] = from_f32<T>(x[e]);
+          for (int u = 0; u < NV; ++u)
+            if (i0 + u * GROUP < left) __stcs(gv + i0 + u * GROUP, v[u]);
+        } else {
+#pragma unroll
+          for (int u = 0; u < NV; ++u) store_elements<T>(v[u], i0 + u * GROUP < left ? gv + i0 + u * GROUP : nullptr);
         }
       };
       if constexpr (RESIDENT) {
-#pragma unroll
-        for (int u = 0; u < NV; ++u)
-          if (u * GROUP < left) put(v[u], u * GROUP);
+        store(0);
       } else {
         for (int i = 0; i < left; i += NV * GROUP) {
 #pragma unroll
           for (int u = 0; u < NV; ++u)
             if (!zero && i + u * GROUP < left) v[u] = load_stream(pv + i + u * GROUP);
-#pragma unroll
-          for (int u = 0; u < NV; ++u)
-            if (i + u * GROUP < left) put(v[u], i + u * GROUP);
+          store(i);
         }
       }
-      if (edge_at >= 0)
-        g[edge_at] = from_f32<T>(zero ? 0.0f : (edge_at == t ? at_t : q * ex2((edge - st.m) * a.t.k)));
+      if (edge_at >= 0) g[edge_at] = from_f32<T>(zero ? 0.0f : q0 * ex2((edge - st.m) * a.t.k));
+      if (hit && !zero) {  // the target's element again, by the thread that wrote it
+        const int j = static_cast<int>(t), i = (j - head) / V;
+        if (j == edge_at || (j >= head && i < nvec && i >= begin && i < begin + per && (i - begin) % GROUP == tid))
+          g[j] = from_f32<T>(fmaf(q0, ex2((target_logit - st.m) * a.t.k), coef));
+      }
     }
     __syncthreads();
-    if (last) {
-      __shared__ double smem[kBlock ? kWarps : 4];
-      __threadfence();
-      double x = 0.0, y = 0.0, z = 0.0;
-      for (int64_t i = threadIdx.x; i < a.t.rows; i += blockDim.x) {
-        const float4 f = __ldcg(a.terms + i);
-        x += f.x;
-        y += f.y;
-        z += f.z;
+    if (last) add_terms<kBlock ? kWarps : 4>(a);
+  }
+}
+
+// ---- long rows: a ring of shared memory between the copies and the arithmetic ---------------------------
+// One block per SM (or a few smaller ones); the grid has a block per row, and a running block takes over rows whose
+// blocks have not started (clusterlaunchcontrol), so that rows that take no part cost nobody a turn.  Three roles that
+// meet at mbarriers only:
+//   copies      one thread fetches the next row's number and copies the row, chunk by chunk, into a ring of SLOTS slots;
+//   arithmetic  CT threads: running maximum and sum of their part of every chunk, then the gradient;
+//   scalars     one warp fetches what the row needs besides its logits while its statistics are made, merges the
+//               warps' parts, and forms the row's log-probability, loss terms and coefficient once for all.
+// A policy row with a gradient is walked twice: its last KEEP chunks stay in the ring for the second walk, the ones in
+// front of them are given back after the statistics and copied again (from L2: the row passed moments before), while
+// the kept ones turn into gradient.  Copies of the next row start as slots fall free.
+constexpr int kRowSlots = 4;  // rows between the copies and the other two
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
+}
+// L2 eviction policies: lines that will be copied again, and lines that will not.
+__device__ __forceinline__ uint64_t l2_keep() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ uint64_t l2_drop() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+
+// Asks for the number of a block of this grid that has not started; the answer (16 bytes) arrives at `bar`.
+__device__ __forceinline__ void next_row_ask(uint4* answer, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(answer)),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// The block's number, or -1 when none is left (then nothing more may be asked).
+__device__ __forceinline__ int64_t next_row_read(const uint4* answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 h;\n\tld.shared.b128 h, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, h;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_u32(answer))
+      : "memory");
+  return got ? static_cast<int64_t>(x) : -1;
+}
+
+template <int SLOTS>
+struct RingPos {
+  int slot = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == SLOTS) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+template <int CT, int VECS, int SLOTS>
+constexpr size_t ring_bytes() {
+  return static_cast<size_t>(SLOTS) * CT * VECS * 16;
+}
+
+template <typename T, int CT, int VECS, int SLOTS, int KEEP, int MODE>
+__global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_kernel(RowArgs a) {
+  constexpr int V = kVec16<T>, kWarps = CT / 32, kChunk = CT * VECS;
+  constexpr int kErr = 0x70;
+  extern __shared__ __align__(128) uint4 ring[];
+  __shared__ uint64_t full[SLOTS], empty[SLOTS], row_full[kRowSlots], row_empty[kRowSlots];
+  __shared__ uint64_t stat_full[2], stat_empty[2], coef_full, asked;
+  __shared__ __align__(16) uint4 answer;
+  __shared__ RowStat stat[2][kWarps];
+  __shared__ float4 row_coef;  // m, coefficient, -coefficient / s, target's logit
+  __shared__ int64_t row_number[kRowSlots], row_target[kRowSlots];
+  __shared__ volatile int abort_flag;
+  __shared__ bool last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cols = static_cast<int>(a.t.cols);
+  const bool want_grad = MODE == kPolicy && a.grad;
+  if (MODE == kStats) pdl_release();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < SLOTS; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], kWarps);
+    }
+    for (int i = 0; i < kRowSlots; ++i) {
+      mbar_init(&row_full[i], 1);
+      mbar_init(&row_empty[i], kWarps + 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&stat_full[i], kWarps);
+      mbar_init(&stat_empty[i], 1);
+    }
+    mbar_init(&coef_full, 1);
+    mbar_init(&asked, 1);
+    abort_flag = 0;
+    last = false;
+    fence_mbar_init();
+    if (MODE == kStats && a.done && blockIdx.x == 0) *a.done = 0;
+  }
+  __syncthreads();
+
+  if (warp == kWarps) {  // ---- rows and copies
+    if (lane == 0) {
+      const uint64_t keep_policy = l2_keep(), drop_policy = l2_drop();
+      RingPos<SLOTS> pos;
+      int64_t issued = 0, r = blockIdx.x;
+      bool ok = true;
+      for (int64_t k = 0; ok; ++k) {
+        const int b = static_cast<int>(k % kRowSlots);
+        int64_t t = a.t.ignore_index;
+        if (r >= 0) {
+          t = a.t.targets[r];
+          if (!a.seq.covers(r)) t = a.t.ignore_index;
+        }
+        if (k >= kRowSlots) ok = mbar_wait(&row_empty[b], static_cast<uint32_t>(k / kRowSlots - 1) & 1, &abort_flag, kErr);
+        if (!ok) break;
+        row_number[b] = r;
+        row_target[b] = t;
+        mbar_arrive(&row_full[b]);
+        if (r < 0) break;
+        mbar_arrive_expect_tx(&asked, 16);
+        next_row_ask(&answer, &asked);
+        if (t != a.t.ignore_index) {
+          const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
+          const int head = static_cast<int>(peel(p, cols)), nvec = (cols - head) / V;
+          const int n = (nvec + kChunk - 1) / kChunk, again = want_grad && n > KEEP ? n - KEEP : 0;
+          const uint4* pv = reinterpret_cast<const uint4*>(p + head);
+          for (int l = 0; l < n + again; ++l) {
+            const int c = l < n ? l : l - n;
+            if (issued >= SLOTS && !mbar_wait(&empty[pos.slot], pos.phase ^ 1, &abort_flag, kErr + 1)) {
+              ok = false;
+              break;
+            }
+            const int vecs = nvec - c * kChunk < kChunk ? nvec - c * kChunk : kChunk;
+            mbar_arrive_expect_tx(&full[pos.slot], vecs * 16);
+            bulk_load(ring + pos.slot * kChunk, pv + static_cast<int64_t>(c) * kChunk, vecs * 16, &full[pos.slot],
+                      l < again ? keep_policy : drop_policy);
+            pos.next();
+            ++issued;
+          }
+        }
+        if (ok) ok = mbar_wait(&asked, static_cast<uint32_t>(k) & 1, &abort_flag, kErr + 2);
+        if (!ok) mbar_wait_drain(&asked, static_cast<uint32_t>(k) & 1, kErr + 2);
+        if (ok) {
+          r = next_row_read(&answer);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the answer is read before the next overwrites it
+        }
       }
-      x = block_sum(x, smem);
-      y = block_sum(y, smem);
-      z = block_sum(z, smem);
-      if (threadIdx.x == 0) {
-        a.out[0] = static_cast<float>(x);
-        a.out[1] = static_cast<float>(y);
-        a.out[2] = static_cast<float>(z);
+      if (!ok) {  // a wait ran out: let the copies in flight land before the block ends
+        const int64_t first = issued > SLOTS ? issued - SLOTS : 0;
+        for (int64_t q = first; q < issued; ++q)
+          mbar_wait_drain(&full[q % SLOTS], static_cast<uint32_t>(q / SLOTS) & 1, kErr + 3);
       }
     }
+    __syncwarp();
+  } else if (warp == kWarps + 1) {  // ---- scalars
+    if (MODE == kPolicy) pdl_wait();
+    int64_t live = 0;  // rows with statistics so far
+    uint32_t counted = 0;
+    for (int64_t k = 0;; ++k) {
+      const int b = static_cast<int>(k % kRowSlots);
+      const bool here = mbar_wait(&row_full[b], static_cast<uint32_t>(k / kRowSlots) & 1, &abort_flag, kErr + 4);
+      if (!__all_sync(0xffffffffu, here)) break;
+      const int64_t r = row_number[b], t = row_target[b];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&row_empty[b]);
+      if (r < 0) break;
+      double lp = 0.0, d = 0.0;
+      float4 term = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      RowStat st{0.0f, 1.0f};
+      if (t != a.t.ignore_index) {
+        const RowScalars sc = load_scalars<T, MODE>(a, r, t);
+        const int h = static_cast<int>(live & 1);
+        const bool made = mbar_wait(&stat_full[h], static_cast<uint32_t>(live >> 1) & 1, &abort_flag, kErr + 5);
+        if (!__all_sync(0xffffffffu, made)) break;
+        st = warp_merge(lane < kWarps ? stat[h][lane] : RowStat{kLowest, 0.0f}, a.t.k);
+        lp = row_logp(a.t, st, sc.target_logit, t);
+        float coef = 0.0f;
+        if constexpr (MODE == kPolicy) term = policy_term(a, sc, lp, coef);
+        d = lp - static_cast<double>(sc.ref);
+        __syncwarp();
+        if (lane == 0) {
+          if (want_grad) {
+            row_coef = make_float4(st.m, coef, coef == 0.0f ? 0.0f : -coef / st.s, sc.target_logit);
+            mbar_arrive(&coef_full);
+          }
+          mbar_arrive(&stat_empty[h]);
+        }
+        ++live;
+      }
+      if (lane == 0) {
+        a.t.logps[r] = static_cast<float>(lp);
+        if constexpr (MODE == kPolicy) {
+          a.terms[r] = term;
+          ++counted;
+        } else {
+          if (a.d) a.d[r] = d;
+          if (a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / st.s, 0.0f, 0.0f);
+        }
+      }
+    }
+    if (MODE == kPolicy && lane == 0) {
+      __threadfence();
+      last = atomicAdd(a.done, counted) + counted == a.t.rows;
+    }
+  } else {  // ---- arithmetic
+    const int tid = threadIdx.x;
+    const uint32_t none = neg_inf_word<T>();
+    const float k2 = a.t.k;
+    RingPos<SLOTS> pos;
+    int64_t live = 0;
+    bool ok = true;
+    for (int64_t k = 0; ok; ++k) {
+      const int b = static_cast<int>(k % kRowSlots);
+      ok = __all_sync(0xffffffffu,
+                      mbar_wait(&row_full[b], static_cast<uint32_t>(k / kRowSlots) & 1, &abort_flag, kErr + 6));
+      if (!ok) break;
+      const int64_t r = row_number[b], t = row_target[b];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&row_empty[b]);
+      if (r < 0) break;
+      const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
+      const int head = static_cast<int>(peel(p, cols)), nvec = (cols - head) / V;
+      const int n = (nvec + kChunk - 1) / kChunk;
+      const int keep = !want_grad ? 0 : (n < KEEP ? n : KEEP);
+      // elements in front of the first and behind the last vector: at most one a thread
+      int edge_at = tid < head ? tid : nvec * V + tid;
+      if (edge_at >= cols) edge_at = -1;
+      if (t == a.t.ignore_index) {  // zeros, whatever the logits hold
+        if (want_grad) {
+          T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
+          const int ghead = static_cast<int>(peel(g, cols)), gvec = (cols - ghead) / V;
+          uint4* gv = reinterpret_cast<uint4*>(g + ghead);
+          for (int i = tid; i < gvec; i += CT) __stcs(gv + i, make_uint4(0, 0, 0, 0));
+          const int j = tid < ghead ? tid : gvec * V + tid;
+          if (j < cols) g[j] = from_f32<T>(0.0f);
+        }
+        continue;
+      }
+      const float edge = edge_at >= 0 ? to_f32(p[edge_at]) : -INFINITY;
+      RowStat st{kLowest, 0.0f};
+      ExpRef ref;
+      ref.set(kLowest, k2);
+      for (int c = 0; c < n && ok; ++c) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&full[pos.slot], pos.phase, &abort_flag, kErr + 7));
+        const uint4* base = ring + pos.slot * kChunk + tid;
+        uint4 v[VECS];
+        if (c < n - 1) {
+#pragma unroll
+          for (int u = 0; u < VECS; ++u) v[u] = base[u * CT];
+        } else {
+          const int left = nvec - c * kChunk - tid;
+#pragma unroll
+          for (int u = 0; u < VECS; ++u) v[u] = u * CT < left ? base[u * CT] : make_uint4(none, none, none, none);
+        }
+        float m = st.m;
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) m = vec_max<T>(v[u], m);
+        if (c < n - keep) {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[pos.slot]);
+        }
+        if (m > st.m) {
+          st.s *= ex2((st.m - m) * k2);
+          st.m = m;
+          ref.set(m, k2);
+        }
+        st.s += vecs_sum<T>(v, ref, k2);
+        pos.next();
+      }
+      const float m = fmaxf(edge, st.m);
+      st.s = st.s * ex2((st.m - m) * k2) + ex2((edge - m) * k2);
+      st.m = m;
+      st = warp_merge(st, k2);
+      const int h = static_cast<int>(live & 1);
+      if (live >= 2)
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&stat_empty[h], static_cast<uint32_t>((live >> 1) - 1) & 1,
+                                                     &abort_flag, kErr + 8));
+      if (!ok) break;
+      if (lane == 0) {
+        stat[h][warp] = st;
+        mbar_arrive(&stat_full[h]);
+      }
+      ++live;
+      if (!want_grad) continue;
+
+      ok = __all_sync(0xffffffffu, mbar_wait(&coef_full, static_cast<uint32_t>(live - 1) & 1, &abort_flag, kErr + 9));
+      if (!ok) break;
+      const float4 f = row_coef;
+      ref.set(f.x, k2);
+      const float coef = f.y, q0 = f.z, q = fmaf(q0, ref.corr, q0);
+      T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
+      uint4* gv = reinterpret_cast<uint4*>(g + head) + tid;
+      const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
+      // the kept chunks n - keep .. n - 1, then 0 .. n - keep - 1 as they arrive again
+      RingPos<SLOTS> at = pos;
+      at.slot = pos.slot >= keep ? pos.slot - keep : pos.slot - keep + SLOTS;
+      for (int l = 0; l < n && ok; ++l) {
+        const int c = l < keep ? n - keep + l : l - keep;
+        if (l == keep) at = pos;
+        if (l >= keep) ok = __all_sync(0xffffffffu, mbar_wait(&full[at.slot], at.phase, &abort_flag, kErr + 10));
+        const uint4* base = ring + at.slot * kChunk + tid;
+        const int left = nvec - c * kChunk - tid;
+        uint4 v[VECS];
+        if (c < n - 1) {
+#pragma unroll
+          for (int u = 0; u < VECS; ++u) v[u] = base[u * CT];
+        } else {
+#pragma unroll
+          for (int u = 0; u < VECS; ++u)
+            if (u * CT < left) v[u] = base[u * CT];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[at.slot]);
+        at.next();
+        uint4* to = gv + static_cast<int64_t>(c) * kChunk;
+        vecs_grad<T>(v, ref, k2, q);
+        if (same) {
+#pragma unroll
+          for (int u = 0; u < VECS; ++u)
+            if (u * CT < left) __stcs(to + u * CT, v[u]);
+        } else {  // the gradient's rows are off the logits' alignment
+#pragma unroll
+          for (int u = 0; u < VECS; ++u) store_elements<T>(v[u], u * CT < left ? to + u * CT : nullptr);
+        }
+      }
+      if (n > keep) pos = at;
+      if (edge_at >= 0) g[edge_at] = from_f32<T>(q0 * ex2((edge - f.x) * k2));
+      // the target's element again, by the thread that wrote it
+      if (t >= 0 && t < cols) {
+        const int j = static_cast<int>(t), i = (j - head) / V;
+        if (j == edge_at || (j >= head && i < nvec && i % CT == tid))
+          g[j] = from_f32<T>(fmaf(q0, ex2((f.w - f.x) * k2), coef));
+      }
+    }
+  }
+  if constexpr (MODE == kPolicy) {
+    __syncthreads();
+    if (last) add_terms<kWarps + 2>(a);
   }
 }
 
@@ -584,10 +974,12 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   const float c = a.slope ? (t == a.t.ignore_index ? 0.0f : a.slope[r] * static_cast<float>(a.t.inv_temp)) : st.z;
   const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
   T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
-  const float q = -c * st.y;
+  ExpRef ref;
+  ref.set(st.x, a.t.k);
+  const float q0 = -c * st.y, q = fmaf(q0, ref.corr, q0);
   const bool zero = c == 0.0f;
   float at_t = 0.0f;
-  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q, ex2((to_f32(p[t]) - st.x) * a.t.k), c);
+  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q0, ex2((to_f32(p[t]) - st.x) * a.t.k), c);
   if (p == g) __syncthreads();
   const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   const int64_t head = same ? peel(g, a.t.cols) : a.t.cols;
@@ -596,36 +988,27 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   const int64_t end = per * (part + 1) < nvec ? per * (part + 1) : nvec;
   const uint4* pv = reinterpret_cast<const uint4*>(p + head);
   uint4* gv = reinterpret_cast<uint4*>(g + head);
-  const int64_t tv = !zero && t >= head && t < tail ? (t - head) / V : -1;
+  const int64_t tv = t >= head && t < tail ? (t - head) / V : -1;
   for (int64_t i0 = per * part + threadIdx.x; i0 < end; i0 += 256 * U) {
     uint4 raw[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (!zero && i0 + u * 256 < end) raw[u] = load_stream(pv + i0 + u * 256);
+    if (zero) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t i = i0 + u * 256;
-      if (i >= end) break;
-      float v[V];
-      if (zero) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = 0.0f;
-      } else {
-        unpack16<T>(raw[u], v);
-#pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = q * ex2((v[e] - st.x) * a.t.k);
-        if (i == tv) {
-#pragma unroll
-          for (int e = 0; e < V; ++e)
-            if (head + i * V + e == t) v[e] = at_t;
-        }
-      }
-      __stcs(gv + i, pack16<T>(v));
+      for (int u = 0; u < U; ++u) raw[u] = make_uint4(0, 0, 0, 0);
+    } else {
+      vecs_grad<T>(raw, ref, a.t.k, q);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (i0 + u * 256 < end) __stcs(gv + i0 + u * 256, raw[u]);
   }
   auto one = [&](int64_t j) {
-    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q * ex2((to_f32(p[j]) - st.x) * a.t.k)));
+    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q0 * ex2((to_f32(p[j]) - st.x) * a.t.k)));
   };
+  // the target's element again, by the thread that wrote it
+  if (!zero && tv >= per * part && tv < end && (tv - per * part) % 256 == threadIdx.x) g[t] = from_f32<T>(at_t);
   if (same) {  // the few elements in front of and behind the vectors
     const int64_t j = static_cast<int64_t>(threadIdx.x) < head ? threadIdx.x : tail + (threadIdx.x - head);
     if (part == 0 && j < a.t.cols) one(j);
@@ -644,60 +1027,58 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* x, int64_t n, const fl
 }
 
 // ---- launchers -------------------------------------------------------------------------------------
-// A launch in clusters of `cluster` blocks; `early`: it may start before the kernel in front of it has ended, and
-// waits (griddepcontrol.wait) where it needs that kernel's results.
-template <typename Args>
-cudaError_t launch_kernel(void (*fn)(Args), int64_t blocks, int threads, int cluster, bool early, const Args& args,
-                          cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-  cfg.blockDim = dim3(static_cast<unsigned>(threads));
-  cfg.stream = stream;
-  cudaLaunchAttribute at[2];
-  int n = 0;
-  if (cluster > 1) {
-    at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n].val.clusterDim.x = static_cast<unsigned>(cluster);
-    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
-    ++n;
+template <typename T, int CT, int VECS, int SLOTS, int KEEP, int MODE>
+cudaError_t launch_ring(const RowArgs& a, bool early, cudaStream_t stream) {
+  auto fn = token_ring_kernel<T, CT, VECS, SLOTS, KEEP, MODE>;
+  constexpr size_t kSmem = ring_bytes<CT, VECS, SLOTS>();
+  // the shared-memory cap is a function attribute of each device
+  static std::atomic<uint64_t> configured[2] = {};
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  if (device < 0 || device >= 128) return cudaErrorInvalidDevice;
+  const uint64_t bit = uint64_t(1) << (device & 63);
+  if (!(configured[device >> 6].load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
+    if (e != cudaSuccess) return e;
+    configured[device >> 6].fetch_or(bit, std::memory_order_release);
   }
-  if (early) {
-    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[n].val.programmaticStreamSerializationAllowed = 1;
-    ++n;
-  }
-  cfg.attrs = at;
-  cfg.numAttrs = static_cast<unsigned>(n);
-  count_launch();
-  return cudaLaunchKernelEx(&cfg, fn, args);
+  return launch_kernel(fn, a.t.rows, CT + 64, 1, early, a, stream, kSmem);
 }
 
-// The row kernel for a row of `vecs` 16-byte vectors: a warp up to 8 vectors a lane, a block of 128 up to 8 a thread,
-// else blocks of 512 in the smallest cluster whose threads hold the row in 10 vectors each; longer rows
-// run through a cluster of 8 twice.  With fewer rows than fill the SMs, a larger cluster shares a row.
+// The kernel for `rows` rows of `vecs` 16-byte vectors (16384 rows, log-probabilities, on one B200):
+//   up to 256 vectors   a warp per row, in registers (1000 fp32: 20 us; a block of 128 per row 35 us)
+//   up to 1024          a warp per row (with a gradient up to 400, the row then read again through the caches;
+//                       2500 fp32: 28 us; the ring 50 us)
+//   longer              the ring: blocks of 128, 4 an SM, up to 150 KB a row (64 KB rows: 83 us; blocks of 512 103 us);
+//                       of 256, 2 an SM, up to 400 KB (304 KB: 86 us; 91 us); of 512 beyond (608 KB: 139 us; 144 us)
+// With too few rows for one each to fill the SMs, a row goes to a block or a cluster of up to 8 blocks of 512 that
+// hold it in registers (10 vectors a thread; longer rows are read twice).
 template <typename T, int MODE>
 cudaError_t launch_rows(const RowArgs& a, bool early, cudaStream_t stream) {
   const int64_t rows = a.t.rows, vecs = (a.t.cols + kVec16<T> - 1) / kVec16<T>;
-  if (vecs <= 32 * 2) return launch_kernel(token_row_kernel<T, 32, 2, true, MODE>, (rows + 3) / 4, 128, 1, early, a, stream);
-  if (vecs <= 32 * 8 && rows > 4 * 148)
-    return launch_kernel(token_row_kernel<T, 32, 8, true, MODE>, (rows + 3) / 4, 128, 1, early, a, stream);
+  const int64_t fours = (rows + 3) / 4;
+  if (vecs <= 64) return launch_kernel(token_row_kernel<T, 32, 2, true, MODE>, fours, 128, 1, early, a, stream);
+  if (rows >= 192) {
+    if (vecs <= 256) return launch_kernel(token_row_kernel<T, 32, 8, true, MODE>, fours, 128, 1, early, a, stream);
+    if (vecs <= (MODE == kPolicy ? 400 : 1024) && rows >= 8 * 148)
+      return launch_kernel(token_row_kernel<T, 32, 4, false, MODE>, fours, 128, 1, early, a, stream);
+    if (vecs <= 9600) return launch_ring<T, 128, 4, 6, 4, MODE>(a, early, stream);
+    if (vecs <= 25600) return launch_ring<T, 256, 4, 6, 4, MODE>(a, early, stream);
+    return launch_ring<T, 512, 4, 6, 4, MODE>(a, early, stream);
+  }
   if (vecs <= 128 * 3) return launch_kernel(token_row_kernel<T, 128, 3, true, MODE>, rows, 128, 1, early, a, stream);
-  if (vecs <= 128 * 8 && rows > 2 * 148)
-    return launch_kernel(token_row_kernel<T, 128, 8, true, MODE>, rows, 128, 1, early, a, stream);
   int cluster = 1;
   while (cluster < kMaxCluster && (vecs > 512 * 10 * cluster || (rows * cluster < 148 && vecs > 1024 * cluster))) cluster *= 2;
-  const int64_t need = (vecs + 512 * cluster - 1) / (512 * cluster);
-  const int64_t blocks = rows * cluster;
+  const int64_t need = (vecs + 512 * cluster - 1) / (512 * cluster), blocks = rows * cluster;
   if (need <= 3) return launch_kernel(token_row_kernel<T, 512, 3, true, MODE>, blocks, 512, cluster, early, a, stream);
-  if (need <= 6) return launch_kernel(token_row_kernel<T, 512, 6, true, MODE>, blocks, 512, cluster, early, a, stream);
-  if (need <= 8) return launch_kernel(token_row_kernel<T, 512, 8, true, MODE>, blocks, 512, cluster, early, a, stream);
   if (need <= 10) return launch_kernel(token_row_kernel<T, 512, 10, true, MODE>, blocks, 512, cluster, early, a, stream);
   return launch_kernel(token_row_kernel<T, 512, 4, false, MODE>, blocks, 512, cluster, early, a, stream);
 }
 
 template <typename T>
 cudaError_t token_logps_t(const RowArgs& a, cudaStream_t stream) {
-  return launch_rows<T, kLogps>(a, false, stream);
+  return launch_rows<T, kStats>(a, false, stream);
 }
 
 template <typename T>
@@ -716,7 +1097,7 @@ cudaError_t logit_grad_t(GradArgs a, bool early, cudaStream_t stream) {
 
 template <typename T>
 cudaError_t preference_loss_t(const RowArgs& rows, const PreferenceArgs& a, const GradArgs& g, cudaStream_t stream) {
-  cudaError_t e = launch_rows<T, kPreference>(rows, false, stream);
+  cudaError_t e = launch_rows<T, kStats>(rows, false, stream);
   if (e == cudaSuccess) e = launch_kernel(preference_pair_kernel, a.seq.count / 2, 256, 1, true, a, stream);
   return e != cudaSuccess || !g.grad ? e : logit_grad_t<T>(g, true, stream);
 }
