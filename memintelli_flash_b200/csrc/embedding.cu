@@ -91,8 +91,8 @@ cudaError_t lookup_t(IntList ids, int64_t n, const void* table, int64_t vocab, i
 // ---- stable radix sort of the ids: up to 65536 tokens in one launch -------------------------------------
 // The blocks of one cluster (8, or a single block for up to 2048 tokens) hold all (id, position) pairs in registers
 // and sort them by up to 9 bits a pass, least significant first: ranks within a warp by match, counts of the warps
-// and blocks added through (distributed) shared memory.  151936 rows take two passes.  The grid's other blocks
-// meanwhile write the dense gradient's zeros, so the sort costs no time of its own next to a large table.
+// and blocks added through (distributed) shared memory.  151936 rows take two passes (16384 tokens: 16 us).  The zeros
+// of a dense gradient are written by a kernel that does not wait for the sort until it has written them.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kBins = 512, kSortCluster = 8;
 
 struct SortArgs {
@@ -101,9 +101,12 @@ struct SortArgs {
   uint32_t *keys0, *keys1, *pos0, *pos1;  // scratch: even passes write 0, odd ones 1
   int32_t passes, bits;
   uint32_t* heads;             // [0]: number of split runs, zeroed here
-  // zeros of the dense gradient
-  void* zero;
-  int64_t zero_rows, zero_row_bytes, zero_pitch;
+};
+
+// A dense gradient to be cleared.
+struct ZeroArgs {
+  void* p;
+  int64_t rows, row_bytes, pitch;
 };
 
 // Ids that add nothing (the padding row's, ids outside the table) take the key `vocab` and end up last.
@@ -111,32 +114,33 @@ __device__ __forceinline__ uint32_t sort_key(int64_t id, int64_t vocab, int64_t 
   return static_cast<uint32_t>(id < 0 || id >= vocab || id == padding ? vocab : id);
 }
 
-__device__ void write_zeros(const SortArgs& a, int64_t block, int64_t blocks) {
-  char* p = static_cast<char*>(a.zero);
-  const int64_t stride = blocks * blockDim.x, first = block * blockDim.x + threadIdx.x;
-  if (a.zero_pitch == a.zero_row_bytes && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-    const int64_t bytes = a.zero_rows * a.zero_row_bytes;
-    for (int64_t i = first; i < bytes / 16; i += stride) reinterpret_cast<uint4*>(p)[i] = make_uint4(0, 0, 0, 0);
-    for (int64_t i = bytes / 16 * 16 + first * 2; i < bytes; i += stride * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
+__global__ void __launch_bounds__(512) zero_kernel(ZeroArgs a) {
+  pdl_release();
+  char* p = static_cast<char*>(a.p);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (a.pitch == a.row_bytes && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
+    const int64_t bytes = a.rows * a.row_bytes, whole = bytes / 16 * 16;
+    uint4* v = reinterpret_cast<uint4*>(p);
+#pragma unroll 4
+    for (int64_t i = first; i < whole / 16; i += stride) v[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = whole + first * 2; i < bytes; i += stride * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
   } else {
-    const int64_t per = a.zero_row_bytes / 2;
-    for (int64_t i = first; i < a.zero_rows * per; i += stride)
-      *reinterpret_cast<uint16_t*>(p + i / per * a.zero_pitch + i % per * 2) = 0;
+    const int64_t per = a.row_bytes / 2;
+    for (int64_t i = first; i < a.rows * per; i += stride)
+      *reinterpret_cast<uint16_t*>(p + i / per * a.pitch + i % per * 2) = 0;
   }
+  pdl_wait();  // the kernel behind this one waits for this one alone, and needs the sort too
 }
 
 template <int ITEMS>
-__global__ void __launch_bounds__(kSortThreads) sort_zero_kernel(SortArgs a) {
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(SortArgs a) {
   __shared__ uint16_t count[kSortWarps][kBins];
   __shared__ uint16_t total[kSortCluster][kBins];
   __shared__ uint32_t base[kBins];
   __shared__ uint32_t warp_sum[kBins / 32];
   pdl_release();
   const uint32_t nranks = cluster_size(), rank = cluster_rank();
-  if (blockIdx.x >= nranks) {
-    write_zeros(a, blockIdx.x - nranks, gridDim.x - nranks);
-    return;
-  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (rank == 0 && threadIdx.x == 0) a.heads[0] = 0;
   if (nranks > 1) cluster_arrive();  // waited for in front of the first remote store
@@ -259,8 +263,6 @@ __global__ void __launch_bounds__(kTileThreads) sort_keys_kernel(IntList ids, in
   if (i == 0) heads[0] = 0;
 }
 
-__global__ void __launch_bounds__(1024) zero_kernel(SortArgs a) { write_zeros(a, blockIdx.x, gridDim.x); }
-
 __global__ void __launch_bounds__(kTileThreads) sort_hist_kernel(const uint32_t* __restrict__ keys, int64_t n, int shift,
                                                                  uint32_t* __restrict__ hist, int blocks) {
   __shared__ uint32_t h[kDigits];
@@ -349,7 +351,7 @@ __global__ void __launch_bounds__(kTileThreads) sort_scatter_kernel(const uint32
 
 // ---- gradient -----------------------------------------------------------------------------------------
 // The sorted positions are cut into chunks; a group of threads, one per column vector, walks its chunk's tokens in
-// order, eight rows in flight, and writes each run that lies inside the chunk.  A run that crosses chunk borders
+// order, eight rows in flight in its part of shared memory, and writes each run that lies inside the chunk.  A run that crosses chunk borders
 // leaves one partial sum per chunk (slot 0 of the chunks it enters, slot 1 of the one it starts in), and its first
 // chunk goes on the list of split runs, which the join kernel adds up, in order.  The cut depends on n alone, so the
 // bits are the same every time.
@@ -408,11 +410,14 @@ __device__ __forceinline__ void write_run(const EmbedGradArgs& a, uint32_t row, 
   store_cols<O, V>(o, s);
 }
 
-// V columns of a row as they are stored.
+// V columns of a row on their way through a thread's own places in shared memory: 16-byte asynchronous copies, or plain
+// loads where rows are off that alignment.
 template <typename G, int V>
-struct RawCols {
+struct Staged {
   using type = uint4;
-  static __device__ __forceinline__ uint4 load(const G* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+  static __device__ __forceinline__ void start(uint4* to, const G* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+  }
   static __device__ __forceinline__ void add(const uint4& u, float (&s)[V]) {
     float v[V];
     unpack16<G>(u, v);
@@ -421,96 +426,127 @@ struct RawCols {
   }
 };
 template <typename G>
-struct RawCols<G, 1> {
+struct Staged<G, 1> {
   using type = G;
-  static __device__ __forceinline__ G load(const G* p) { return __ldg(p); }
+  static __device__ __forceinline__ void start(G* to, const G* from) { *to = *from; }
   static __device__ __forceinline__ void add(G u, float (&s)[1]) { s[0] += to_f32(u); }
 };
 
 template <typename G, typename O, int V>
 __global__ void __launch_bounds__(256) embed_sum_kernel(EmbedGradArgs a) {
-  constexpr int U = 8;
+  constexpr int kAhead = 8;  // rows in flight
+  using S = Staged<G, V>;
+  __shared__ typename S::type stage[kAhead + 1][256];
   pdl_release();
   pdl_wait();
   const int64_t col = (static_cast<int64_t>(blockIdx.y) * blockDim.x + threadIdx.x) * V;
   const int64_t c = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
-  const int64_t begin = c * a.chunk, end = begin + a.chunk < a.n ? begin + a.chunk : a.n;
-  if (begin >= a.n || col >= a.hidden) return;
+  const int64_t begin = c * a.chunk;
+  if (begin >= a.n) return;  // the whole warp: a row of threads is a multiple of 32
+  const int len = static_cast<int>(a.n - begin < a.chunk ? a.n - begin : a.chunk);  // at most 64
+  const bool mine = col < a.hidden;
+  const int tid = threadIdx.y * blockDim.x + threadIdx.x, lane = tid & 31;
   const uint32_t none = static_cast<uint32_t>(a.vocab);
-  const uint32_t in = begin > 0 ? __ldcg(a.keys + begin - 1) : none;  // the key in front of the chunk
-  const uint32_t out = end < a.n ? __ldcg(a.keys + end) : none;       // the one behind it
-  const G* grad = static_cast<const G*>(a.grad) + col;
-  uint32_t run = __ldcg(a.keys + begin);
+  // the chunk's keys and positions, two a lane, and the keys in front of it and behind it
+  uint32_t key[2], pos[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t = h * 32 + lane;
+    key[h] = t < len ? __ldcg(a.keys + begin + t) : none;
+    pos[h] = t < len ? __ldcg(a.pos + begin + t) : 0;
+  }
+  const uint32_t in = begin > 0 ? __ldcg(a.keys + begin - 1) : none;
+  const uint32_t out = begin + len < a.n ? __ldcg(a.keys + begin + len) : none;
+  const G* grad = static_cast<const G*>(a.grad) + (mine ? col : 0);
+  auto key_at = [&](int t) { return __shfl_sync(0xffffffffu, t < 32 ? key[0] : key[1], t & 31); };
+  auto start = [&](int t, int slot) {
+    if (t < len) {
+      const uint32_t p = __shfl_sync(0xffffffffu, t < 32 ? pos[0] : pos[1], t & 31);
+      if (key_at(t) != none && mine) S::start(&stage[slot][tid], grad + static_cast<int64_t>(p) * a.ld_grad);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int t = 0; t < kAhead; ++t) start(t, t);
+  uint32_t run = key_at(0);
   bool entered = run == in;  // the run began in an earlier chunk
   float s[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) s[e] = 0.0f;
-  for (int64_t i0 = begin; i0 < end && run != none; i0 += U) {
-    uint32_t key[U];
-    typename RawCols<G, V>::type v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) key[u] = i0 + u < end ? __ldcg(a.keys + i0 + u) : none;
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (key[u] != none) v[u] = RawCols<G, V>::load(grad + static_cast<int64_t>(__ldcg(a.pos + i0 + u)) * a.ld_grad);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (i0 + u >= end) break;
-      if (key[u] != run) {  // uniform over the chunk's threads
+  int slot = 0;
+#pragma unroll 1
+  for (int t = 0; t < len; ++t) {
+    const uint32_t k = key_at(t);  // uniform over the chunk's threads
+    if (k != run) {
+      if (mine) {
         if (entered) store_cols<float, V>(a.partial + (2 * c) * a.hidden + col, s);
         else write_run<O, V>(a, run, col, s);
-        entered = false;
-        run = key[u];
-#pragma unroll
-        for (int e = 0; e < V; ++e) s[e] = 0.0f;
-        if (run == none) break;
       }
-      RawCols<G, V>::add(v[u], s);
+      entered = false;
+      run = k;
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] = 0.0f;
     }
+    if (run == none) break;
+    asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+    if (mine) S::add(stage[slot][tid], s);
+    start(t + kAhead, slot == 0 ? kAhead : slot - 1);  // the place that the row before had
+    slot = slot == kAhead ? 0 : slot + 1;
   }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (run == none) return;
-  if (entered) {
-    store_cols<float, V>(a.partial + (2 * c) * a.hidden + col, s);
-  } else if (run == out) {
-    store_cols<float, V>(a.partial + (2 * c + 1) * a.hidden + col, s);
+  if (!entered && run == out) {
+    if (mine) store_cols<float, V>(a.partial + (2 * c + 1) * a.hidden + col, s);
     if (blockIdx.y == 0 && threadIdx.x == 0) a.heads[1 + atomicAdd(a.heads, 1u)] = static_cast<uint32_t>(c);
-  } else {
-    write_run<O, V>(a, run, col, s);
+  } else if (mine) {
+    if (entered) store_cols<float, V>(a.partial + (2 * c) * a.hidden + col, s);
+    else write_run<O, V>(a, run, col, s);
   }
 }
 
-// Adds up the split runs: 32 columns and 8 stretches of a run's chunks per block, the stretches' sums joined in order.
-template <typename O>
+// Adds up the split runs: 32 column vectors and 8 stretches of a run's chunks per block, the stretches' sums joined
+// in order.
+template <typename O, int V>
 __global__ void __launch_bounds__(256) embed_join_kernel(EmbedGradArgs a) {
-  __shared__ float part[8][33];
+  __shared__ float part[8][V][33];
   pdl_wait();
   const int lane = threadIdx.x & 31, g = threadIdx.x >> 5;
-  const int64_t col = static_cast<int64_t>(blockIdx.y) * 32 + lane;
-  const uint32_t count = __ldcg(a.heads);
+  const uint32_t tiles = static_cast<uint32_t>((a.hidden + 32 * V - 1) / (32 * V)), count = __ldcg(a.heads) * tiles;
+  const int64_t chunks = (a.n + a.chunk - 1) / a.chunk;
   for (uint32_t h = blockIdx.x; h < count; h += gridDim.x) {
-    const int64_t c = __ldcg(a.heads + 1 + h);
+    const int64_t c = __ldcg(a.heads + 1 + h / tiles), col = (static_cast<int64_t>(h % tiles) * 32 + lane) * V;
     const uint32_t run = __ldcg(a.keys + (c + 1) * a.chunk);
-    // the run's last chunk: the one that holds its last position
-    int64_t lo = (c + 1) * a.chunk, hi = a.n;  // keys[lo] == run; first position past the run in (lo, hi]
-    while (hi - lo > 1) {
-      const int64_t mid = (lo + hi) / 2;
-      if (__ldcg(a.keys + mid) == run) lo = mid; else hi = mid;
+    // chunks c + 1 .. c + m hold the rest, in their slot 0: those whose first key is still the run's
+    int64_t m = 1;
+    for (;;) {
+      const int64_t at = c + 1 + m + lane;
+      const uint32_t same = __ballot_sync(0xffffffffu, at < chunks && __ldcg(a.keys + at * a.chunk) == run);
+      m += same == 0xffffffffu ? 32 : __ffs(~same) - 1;
+      if (same != 0xffffffffu) break;
     }
-    const int64_t m = lo / a.chunk - c;  // chunks c + 1 .. c + m hold the rest in their slot 0
     const int64_t per = (m + 7) / 8, first = g * per, last = first + per < m ? first + per : m;
-    float s = 0.0f;
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.0f;
     if (col < a.hidden) {
       const float* p = a.partial + col;
-      if (g == 0) s = __ldcg(p + (2 * c + 1) * a.hidden);
-#pragma unroll 8
-      for (int64_t i = first; i < last; ++i) s += __ldcg(p + 2 * (c + 1 + i) * a.hidden);
+      if (g == 0) load_cols<float, V>(p + (2 * c + 1) * a.hidden, s);
+#pragma unroll 4
+      for (int64_t i = first; i < last; ++i) {
+        float v[V];
+        load_cols<float, V>(p + 2 * (c + 1 + i) * a.hidden, v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] += v[e];
+      }
     }
-    part[g][lane] = s;
+#pragma unroll
+    for (int e = 0; e < V; ++e) part[g][e][lane] = s[e];
     __syncthreads();
     if (g == 0 && col < a.hidden) {
-      float t[1] = {part[0][lane]};
-      for (int w = 1; w < 8; ++w) t[0] += part[w][lane];
-      write_run<O, 1>(a, run, col, t);
+      for (int w = 1; w < 8; ++w)
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[e] += part[w][e][lane];
+      write_run<O, V>(a, run, col, s);
     }
     __syncthreads();
   }
@@ -568,10 +604,6 @@ cudaError_t sort_tiles(const SortArgs& s, const EmbedPlan& p, uint32_t* hist, cu
     sort_scatter_kernel<<<blocks, kTileThreads, 0, stream>>>(keys_in, pos_in, s.n, 8 * q, hist, b, keys_out, pos_out);
     count_launch(3);
   }
-  if (s.zero_rows > 0) {
-    zero_kernel<<<148, 1024, 0, stream>>>(s);
-    count_launch();
-  }
   return cudaGetLastError();
 }
 
@@ -593,9 +625,11 @@ cudaError_t embed_sum_v(const EmbedGradArgs& a, const EmbedPlan& p, cudaStream_t
   cudaError_t e = cudaLaunchKernelEx(&cfg, embed_sum_kernel<G, O, V>, a);
   if (e != cudaSuccess || p.chunks == 1) return e;
   cfg.blockDim = dim3(256);
-  cfg.gridDim = dim3(static_cast<unsigned>(p.chunks < 64 ? p.chunks : 64), static_cast<unsigned>((a.hidden + 31) / 32));
+  constexpr int W = V == 1 ? 1 : kVec16<O>;
+  const int64_t most = p.chunks * ((a.hidden + 32 * W - 1) / (32 * W));
+  cfg.gridDim = dim3(static_cast<unsigned>(most < 148 * 8 ? most : 148 * 8));
   count_launch();
-  return cudaLaunchKernelEx(&cfg, embed_join_kernel<O>, a);
+  return cudaLaunchKernelEx(&cfg, embed_join_kernel<O, W>, a);
 }
 
 template <typename G, typename O>
@@ -614,21 +648,17 @@ cudaError_t embed_grad_t(EmbedGradArgs a, SortArgs s, void* workspace, cudaStrea
   s.bits = p.bits;
   a.keys = (p.passes & 1) ? s.keys0 : s.keys1;
   a.pos = (p.passes & 1) ? s.pos0 : s.pos1;
-  s.zero = a.out;
-  s.zero_rows = a.accumulate ? 0 : a.vocab;
-  s.zero_row_bytes = a.hidden * static_cast<int64_t>(sizeof(O));
-  s.zero_pitch = a.ld_out * static_cast<int64_t>(sizeof(O));
   cudaError_t e;
   if (p.items == 0) {
     e = sort_tiles(s, p, reinterpret_cast<uint32_t*>(ws + p.hist), stream);
   } else {
-    // blocks that write zeros: 64 KB each, at most the SMs that the sort leaves
-    int64_t fill = (s.zero_rows * s.zero_row_bytes + 65535) / 65536;
-    if (fill > 136) fill = 136;
-    const int64_t blocks = p.cluster + (fill + p.cluster - 1) / p.cluster * p.cluster;
-    auto fn = p.items == 1 ? sort_zero_kernel<1>
-                           : (p.items == 2 ? sort_zero_kernel<2> : (p.items == 4 ? sort_zero_kernel<4> : sort_zero_kernel<8>));
-    e = launch_kernel(fn, blocks, kSortThreads, p.cluster, false, s, stream);
+    auto fn = p.items == 1 ? sort_kernel<1> : (p.items == 2 ? sort_kernel<2> : (p.items == 4 ? sort_kernel<4> : sort_kernel<8>));
+    e = launch_kernel(fn, p.cluster, kSortThreads, p.cluster, false, s, stream);
+  }
+  if (e == cudaSuccess && !a.accumulate) {
+    const ZeroArgs z{a.out, a.vocab, a.hidden * static_cast<int64_t>(sizeof(O)), a.ld_out * static_cast<int64_t>(sizeof(O))};
+    const int64_t want = (z.rows * z.row_bytes + 32767) / 32768;  // 4 vectors a thread, up to 4 blocks an SM
+    e = launch_kernel(zero_kernel, want < 148 * 4 ? want : 148 * 4, 512, 1, true, z, stream);
   }
   if (e != cudaSuccess) return e;
   constexpr int V = kVec16<G>;

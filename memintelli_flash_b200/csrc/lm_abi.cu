@@ -298,7 +298,7 @@ int mib_clip_grad_norm_workspace(int32_t count, int64_t* bytes_out) {
   if (!bytes_out) return fail(MIB_ERR_PARAM, "NULL argument");
   if (count < 0) return fail(MIB_ERR_SHAPE, "negative tensor count");
   const int64_t launches = (static_cast<int64_t>(count) + mib::kClipTensors - 1) / mib::kClipTensors;
-  *bytes_out = align256(launches * mib::kClipBlocks * 8) + 256;
+  *bytes_out = align256((launches + 1) * mib::kClipBlocks * 8);
   return MIB_OK;
 }
 
@@ -311,7 +311,7 @@ int mib_clip_grad_norm(const void* const* in, void* const* out, const int64_t* n
   if (out && (!(max_norm >= 0.0f) || !(eps >= 0.0f))) return fail(MIB_ERR_PARAM, "max_norm must be non-negative");
   bool in_place = out != nullptr;
   for (int32_t i = 0; i < count; ++i) {
-    if (numel[i] < 0 || numel[i] > (int64_t(1) << 40)) return fail(MIB_ERR_SHAPE, "invalid tensor size");
+    if (numel[i] < 0 || numel[i] > (int64_t(1) << 42)) return fail(MIB_ERR_SHAPE, "invalid tensor size");
     if (!known_dtype(in_dtype[i]) || (out && !known_dtype(out_dtype[i])))
       return fail(MIB_ERR_UNSUPPORTED, "gradients must be fp32, bf16 or fp16");
     if (numel[i] > 0 && (!in[i] || (out && !out[i]))) return fail(MIB_ERR_PARAM, "NULL tensor");
@@ -325,49 +325,35 @@ int mib_clip_grad_norm(const void* const* in, void* const* out, const int64_t* n
   s.max_norm = max_norm;
   s.eps = eps;
   s.norm = norm;
-  s.coef = out ? reinterpret_cast<float*>(static_cast<char*>(workspace) + need - 256) : nullptr;
-
-  mib::ClipTable t;
-  for (int pass = 0; pass < (out ? 2 : 1); ++pass) {
-    int32_t i = 0;
-    while (i < count) {
-      t.count = 0;
-      t.first[0] = 0;
-      for (; i < count && t.count < mib::kClipTensors; ++i) {
-        if (numel[i] == 0) continue;
-        const int64_t chunks = (numel[i] + mib::kClipChunk - 1) / mib::kClipChunk;
-        if (t.first[t.count] + chunks > (int64_t(1) << 30)) {
-          if (t.count == 0) return fail(MIB_ERR_SHAPE, "tensor too large");
-          break;
-        }
-        const int k = t.count++;
-        t.in[k] = in[i];
-        t.out[k] = out ? out[i] : nullptr;
-        t.numel[k] = numel[i];
-        t.in_type[k] = static_cast<uint8_t>(in_dtype[i]);
-        t.out_type[k] = static_cast<uint8_t>(out ? out_dtype[i] : 0);
-        t.first[k + 1] = t.first[k] + static_cast<int32_t>(chunks);
-      }
-      if (t.count == 0) break;
-      cudaError_t e;
-      if (pass == 0) {
-        s.part_first = s.part_total;
-        s.part_total += static_cast<int32_t>(mib::clip_grid(t));
-        if (static_cast<int64_t>(s.part_total) * 8 > need - 256) return fail(MIB_ERR_SHAPE, "tensor list too large");
-        e = norm_type == 2 ? mib::clip_norm_p<2>(t, s, stream)
-                           : (norm_type == 1 ? mib::clip_norm_p<1>(t, s, stream) : mib::clip_norm_p<0>(t, s, stream));
-      } else {
-        e = mib::clip_scale(t, s.coef, in_place, stream);
-      }
-      if (e != cudaSuccess) return cuda_fail(e, "clip_grad_norm launch");
-    }
-    if (pass == 0) {
-      const cudaError_t e = norm_type == 2 ? mib::clip_finish_p<2>(s, stream)
-                                           : (norm_type == 1 ? mib::clip_finish_p<1>(s, stream) : mib::clip_finish_p<0>(s, stream));
-      if (e != cudaSuccess) return cuda_fail(e, "clip_grad_norm launch");
-    }
+  // calls f with the norm's kind as a compile-time constant
+  auto by_norm = [&](auto f) {
+    if (norm_type == 2) return f(std::integral_constant<int, 2>());
+    if (norm_type == 1) return f(std::integral_constant<int, 1>());
+    return f(std::integral_constant<int, 0>());
+  };
+  const cudaError_t ok = cudaSuccess;
+  cudaError_t e = ok;
+  int launches = 0;
+  int r = mib::clip_tables(in, out, numel, in_dtype, out_dtype, count, [&](const mib::ClipTable& t) {
+    s.part_first = s.part_total;
+    s.part_total += static_cast<int32_t>(mib::clip_grid(t));
+    if (static_cast<int64_t>(s.part_total) * 8 > need) return fail(MIB_ERR_SHAPE, "tensor list too large");
+    e = by_norm([&](auto p) { return mib::clip_norm_p<decltype(p)::value>(t, s, stream); });
+    ++launches;
+    return e == ok ? MIB_OK : cuda_fail(e, "clip_grad_norm launch");
+  });
+  if (r) return r;
+  if (!out || launches == 0) {
+    e = by_norm([&](auto p) { return mib::clip_finish_p<decltype(p)::value>(s, stream); });
+    return e == ok ? MIB_OK : cuda_fail(e, "clip_grad_norm launch");
   }
-  return MIB_OK;
+  // the scaling may start early only behind the one launch that it waits for
+  bool early = launches == 1;
+  return mib::clip_tables(in, out, numel, in_dtype, out_dtype, count, [&](const mib::ClipTable& t) {
+    e = by_norm([&](auto p) { return mib::clip_scale_p<decltype(p)::value>(t, s, in_place, early, stream); });
+    early = false;
+    return e == ok ? MIB_OK : cuda_fail(e, "clip_grad_norm launch");
+  });
 }
 
 }  // extern "C"

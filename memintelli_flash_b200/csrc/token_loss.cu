@@ -906,47 +906,57 @@ __device__ __forceinline__ void preference_term(const PreferenceArgs& a, double 
   }
 }
 
-// One block per pair: the sums of both sequences, the pair's loss, and the coefficient of their rows.
-__global__ void __launch_bounds__(256) preference_pair_kernel(PreferenceArgs a) {
-  __shared__ double smem[8];
+// One block per pair, one half of it per sequence: the sums of both, the pair's loss, and the coefficient of their rows
+// (of all of them: rows that take no part are the gradient's to leave out).
+__global__ void __launch_bounds__(512) preference_pair_kernel(PreferenceArgs a) {
+  __shared__ double part[2][8], counted[2][8], smem[16];
   pdl_release();
-  pdl_wait();
   const int64_t pairs = a.seq.count / 2, i = blockIdx.x;
-  double d[2], n[2];
-  for (int side = 0; side < 2; ++side) {
-    const int64_t s = i + side * pairs;
-    const int64_t lo = a.seq.begin(s, a.t.rows), hi = a.seq.begin(s + 1, a.t.rows);
-    double x = 0.0, c = 0.0;
-    for (int64_t r = lo + threadIdx.x; r < hi; r += 256) {
-      x += __ldcg(a.d + r);
-      c += a.t.targets[r] != a.t.ignore_index ? 1.0 : 0.0;
+  const int side = threadIdx.x >> 8, lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) & 7, tid = threadIdx.x & 255;
+  const int64_t s = i + side * pairs;
+  const int64_t lo = a.seq.begin(s, a.t.rows), hi = a.seq.begin(s + 1, a.t.rows);
+  double c = 0.0, x = 0.0;
+  if (a.average)
+    for (int64_t r = lo + tid; r < hi; r += 256) c += a.t.targets[r] != a.t.ignore_index ? 1.0 : 0.0;
+  pdl_wait();
+  for (int64_t r = lo + tid; r < hi; r += 256) x += __ldcg(a.d + r);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x += __shfl_xor_sync(0xffffffffu, x, o);
+    c += __shfl_xor_sync(0xffffffffu, c, o);
+  }
+  if (lane == 0) {
+    part[side][warp] = x;
+    counted[side][warp] = c;
+  }
+  __syncthreads();
+  double d[2] = {0.0, 0.0}, n[2] = {0.0, 0.0};
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    for (int w = 0; w < 8; ++w) {
+      d[q] += part[q][w];
+      n[q] += counted[q][w];
     }
-    d[side] = block_sum(x, smem);
-    n[side] = a.average ? block_sum(c, smem) : 1.0;
-    if (a.average) d[side] = n[side] > 0.0 ? d[side] / n[side] : 0.0;
+    if (!a.average) n[q] = 1.0;
+    d[q] = n[q] > 0.0 ? d[q] / n[q] : 0.0;
   }
   double loss, slope;
   preference_term(a, a.beta * (d[0] - d[1]) - a.margin, loss, slope);
+  if (a.t.row) {
+    double k = slope * a.beta * a.t.inv_temp / static_cast<double>(pairs);
+    if (n[side] > 0.0) k /= n[side];
+    for (int64_t r = lo + tid; r < hi; r += 256) a.t.row[r].z = static_cast<float>(side ? -k : k);
+  }
   if (threadIdx.x == 0) {
     a.chosen[i] = static_cast<float>(a.beta * d[0]);
     a.rejected[i] = static_cast<float>(a.beta * d[1]);
     a.sums[i] = loss;
   }
-  if (a.t.row) {
-    for (int side = 0; side < 2; ++side) {
-      const int64_t s = i + side * pairs;
-      const int64_t lo = a.seq.begin(s, a.t.rows), hi = a.seq.begin(s + 1, a.t.rows);
-      double c = slope * a.beta * a.t.inv_temp / static_cast<double>(pairs);
-      if (n[side] > 0.0) c /= n[side];
-      for (int64_t r = lo + threadIdx.x; r < hi; r += 256)
-        if (a.t.targets[r] != a.t.ignore_index) a.t.row[r].z = static_cast<float>(side ? -c : c);
-    }
-  }
   if (last_block(a.done, gridDim.x)) {
-    double x = 0.0;
-    for (int64_t b = threadIdx.x; b < gridDim.x; b += 256) x += __ldcg(a.sums + b);
-    x = block_sum(x, smem);
-    if (threadIdx.x == 0) *a.out = static_cast<float>(x / static_cast<double>(pairs));
+    double t = 0.0;
+    for (int64_t b = threadIdx.x; b < gridDim.x; b += 512) t += __ldcg(a.sums + b);
+    t = block_sum(t, smem);
+    if (threadIdx.x == 0) *a.out = static_cast<float>(t / static_cast<double>(pairs));
   }
 }
 
@@ -966,12 +976,12 @@ struct GradArgs {
 template <typename T>
 __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   constexpr int V = kVec16<T>, U = 4;
-  pdl_wait();
   const int64_t r = a.t.rows - 1 - blockIdx.x / a.parts;
   const int part = blockIdx.x % a.parts;
-  const float4 st = __ldcg(a.t.row + r);
   const int64_t t = a.t.targets[r];
-  const float c = a.slope ? (t == a.t.ignore_index ? 0.0f : a.slope[r] * static_cast<float>(a.t.inv_temp)) : st.z;
+  pdl_wait();
+  const float4 st = __ldcg(a.t.row + r);
+  const float c = t == a.t.ignore_index ? 0.0f : (a.slope ? a.slope[r] * static_cast<float>(a.t.inv_temp) : st.z);
   const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
   T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
   ExpRef ref;
@@ -1098,7 +1108,7 @@ cudaError_t logit_grad_t(GradArgs a, bool early, cudaStream_t stream) {
 template <typename T>
 cudaError_t preference_loss_t(const RowArgs& rows, const PreferenceArgs& a, const GradArgs& g, cudaStream_t stream) {
   cudaError_t e = launch_rows<T, kStats>(rows, false, stream);
-  if (e == cudaSuccess) e = launch_kernel(preference_pair_kernel, a.seq.count / 2, 256, 1, true, a, stream);
+  if (e == cudaSuccess) e = launch_kernel(preference_pair_kernel, a.seq.count / 2, 512, 1, true, a, stream);
   return e != cudaSuccess || !g.grad ? e : logit_grad_t<T>(g, true, stream);
 }
 
