@@ -19,32 +19,38 @@ def _workspace_bytes(n, vocab, hidden):
     return b.value
 
 
-def _check_ids(ids, device):
-    if ids.dtype not in _INTS:
+def _check_ids(ids, index):
+    """(ids, 1 if they are int64): dense, on CUDA device ``index``."""
+    wide = _INTS.get(ids.dtype)
+    if wide is None:
         raise ValueError(f"ids must be int32 or int64, got {ids.dtype}")
-    if ids.device != device:
-        raise ValueError(f"ids is on {ids.device}, the embedding on {device}")
-    return ids if ids.is_contiguous() else ids.contiguous()
+    if ids.get_device() != index:
+        raise ValueError(f"ids is on {ids.device}, the embedding on cuda:{index}")
+    return (ids if ids.is_contiguous() else ids.contiguous()), wide
 
 
 def _lookup(ids, weight, scale):
-    if not weight.is_cuda:
+    index = weight.get_device()
+    if index < 0:
         raise ValueError("the embedding must be on a CUDA device")
-    if weight.dtype not in _DTYPES:
+    dtype = _DTYPES.get(weight.dtype)
+    if dtype is None:
         raise ValueError(f"the embedding must be float32, bfloat16 or float16, got {weight.dtype}")
-    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+    shape = weight.shape
+    if len(shape) != 2 or not shape[0] or not shape[1]:
         raise ValueError("the embedding must be (rows, columns) and non-empty")
-    if weight.shape[1] > 1 and weight.stride(1) != 1 or weight.shape[0] > 1 and weight.stride(0) < weight.shape[1]:
+    vocab, hidden = shape
+    ld, unit = weight.stride()
+    if vocab == 1:
+        ld = hidden
+    if hidden > 1 and unit != 1 or ld < hidden:
         raise ValueError("the embedding's rows must be dense")
-    dev = weight.device
-    ids = _check_ids(ids, dev)
-    vocab, hidden = weight.shape
-    out = torch.empty(ids.shape + (hidden,), dtype=weight.dtype, device=dev)
+    ids, wide = _check_ids(ids, index)
+    out = weight.new_empty((*ids.shape, hidden))
     n = ids.numel()
     if n:
-        with N.device_guard(dev):
-            N.call("mib_embedding_lookup", ids.data_ptr(), _INTS[ids.dtype], n, weight.data_ptr(), _DTYPES[weight.dtype],
-                   vocab, hidden, weight.stride(0) if vocab > 1 else hidden, scale, out.data_ptr(), N.stream_ptr(dev))
+        N.launch("mib_embedding_lookup", index, ids.data_ptr(), wide, n, weight.data_ptr(), dtype, vocab, hidden, ld,
+                 scale, out.data_ptr())
     return out
 
 
@@ -56,41 +62,50 @@ def embedding_scaled_grad(ids, grad_output, num_embeddings, scale=1.0, *, paddin
     ``grad_output``'s type; ``out`` takes it instead (that type or fp32, rows dense).  With ``accumulate`` the sums are
     added to ``out`` and only the rows of tokens that occur are touched.  ``padding_idx``'s tokens add nothing, nor do
     ids outside the table."""
-    dev = grad_output.device
-    if dev.type != "cuda":
+    index = grad_output.get_device()
+    if index < 0:
         raise ValueError("grad_output must be on a CUDA device")
-    if grad_output.dtype not in _DTYPES:
+    dtype = _DTYPES.get(grad_output.dtype)
+    if dtype is None:
         raise ValueError(f"grad_output must be float32, bfloat16 or float16, got {grad_output.dtype}")
-    if grad_output.dim() != ids.dim() + 1 or grad_output.shape[:-1] != ids.shape or grad_output.shape[-1] < 1:
-        raise ValueError(f"grad_output has shape {tuple(grad_output.shape)}, expected {tuple(ids.shape)} + (H,)")
+    shape = grad_output.shape
+    if shape[:-1] != ids.shape or len(shape) != ids.dim() + 1 or shape[-1] < 1:
+        raise ValueError(f"grad_output has shape {tuple(shape)}, expected {tuple(ids.shape)} + (H,)")
     if num_embeddings < 1:
         raise ValueError("num_embeddings must be positive")
-    if padding_idx is not None and not 0 <= padding_idx < num_embeddings:
+    if padding_idx is None:
+        padding_idx = -1
+    elif not 0 <= padding_idx < num_embeddings:
         raise ValueError("padding_idx must be a row of the table")
-    hidden = grad_output.shape[-1]
+    hidden = shape[-1]
+    ld_out, out_dtype = hidden, dtype
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
-        out = torch.empty(num_embeddings, hidden, dtype=grad_output.dtype, device=dev)
-    elif out.shape != (num_embeddings, hidden) or out.device != dev or out.dtype not in (grad_output.dtype, torch.float32):
-        raise ValueError("out must be (num_embeddings, H) on grad_output's device, of its type or float32")
-    elif hidden > 1 and out.stride(1) != 1 or num_embeddings > 1 and out.stride(0) < hidden:
-        raise ValueError("out's rows must be dense and apart")
-    ids = _check_ids(ids, dev)
+        out = grad_output.new_empty((num_embeddings, hidden))
+    else:
+        out_dtype = _DTYPES.get(out.dtype)
+        if out.shape != (num_embeddings, hidden) or out.get_device() != index or out_dtype not in (dtype, N.F32):
+            raise ValueError("out must be (num_embeddings, H) on grad_output's device, of its type or float32")
+        if num_embeddings > 1:
+            ld_out = out.stride(0)
+        if hidden > 1 and out.stride(1) != 1 or ld_out < hidden:
+            raise ValueError("out's rows must be dense and apart")
+    ids, wide = _check_ids(ids, index)
     n = ids.numel()
     if n == 0:
         return out if accumulate else out.zero_()
-    g = grad_output.detach()
-    g = g if g.dim() == 2 else g.reshape(n, hidden)
-    if hidden > 1 and g.stride(1) != 1 or n > 1 and g.stride(0) < hidden:
-        g = g.contiguous()
+    g, ld = grad_output, hidden
+    if not g.is_contiguous():
+        g = g.detach()
+        g = g if g.dim() == 2 else g.reshape(n, hidden)
+        if hidden > 1 and g.stride(1) != 1 or n > 1 and g.stride(0) < hidden:
+            g = g.contiguous()
+        ld = g.stride(0) if n > 1 else hidden
     nbytes = _workspace_bytes(n, num_embeddings, hidden)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with N.device_guard(dev):
-        N.call("mib_embedding_grad", ids.data_ptr(), _INTS[ids.dtype], n, g.data_ptr(), _DTYPES[g.dtype],
-               g.stride(0) if n > 1 else hidden, num_embeddings, hidden, scale, -1 if padding_idx is None else padding_idx,
-               out.data_ptr(), _DTYPES[out.dtype], out.stride(0) if num_embeddings > 1 else hidden,
-               1 if accumulate else 0, ws.data_ptr(), nbytes, N.stream_ptr(dev))
+    ws = g.new_empty(nbytes, dtype=torch.uint8)
+    N.launch("mib_embedding_grad", index, ids.data_ptr(), wide, n, g.data_ptr(), dtype, ld, num_embeddings, hidden, scale,
+             padding_idx, out.data_ptr(), out_dtype, ld_out, 1 if accumulate else 0, ws.data_ptr(), nbytes)
     return out
 
 

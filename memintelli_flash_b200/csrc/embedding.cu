@@ -120,11 +120,14 @@ __global__ void __launch_bounds__(512) zero_kernel(ZeroArgs a) {
   const int64_t stride = static_cast<int64_t>(gridDim.x) * blockDim.x;
   const int64_t first = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   if (a.pitch == a.row_bytes && reinterpret_cast<uintptr_t>(p) % 16 == 0) {
-    const int64_t bytes = a.rows * a.row_bytes, whole = bytes / 16 * 16;
+    const int64_t bytes = a.rows * a.row_bytes, vecs = bytes / 16;
     uint4* v = reinterpret_cast<uint4*>(p);
-#pragma unroll 4
-    for (int64_t i = first; i < whole / 16; i += stride) v[i] = make_uint4(0, 0, 0, 0);
-    for (int64_t i = whole + first * 2; i < bytes; i += stride * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 2048 + threadIdx.x; i0 < vecs; i0 += gridDim.x * 2048ll) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (i0 + u * 512 < vecs) v[i0 + u * 512] = make_uint4(0, 0, 0, 0);
+    }
+    for (int64_t i = vecs * 16 + first * 2; i < bytes; i += stride * 2) *reinterpret_cast<uint16_t*>(p + i) = 0;
   } else {
     const int64_t per = a.row_bytes / 2;
     for (int64_t i = first; i < a.rows * per; i += stride)
@@ -557,7 +560,7 @@ struct EmbedPlan {
   int64_t blocks, chunk, chunks;
   size_t keys, hist, heads, partial, bytes;
 };
-// Chunks of 8 to 64 tokens, about 512 of them.
+// Chunks of 8 to 64 tokens, for about 512 blocks of 256 threads, a thread per four columns.
 EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t hidden) {
   EmbedPlan p{};
   int width = 1;
@@ -573,7 +576,8 @@ EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t hidden) {
     p.passes = (width + 7) / 8;
   }
   p.chunk = 8;
-  while (p.chunk < 64 && n > p.chunk * 512) p.chunk *= 2;
+  const int64_t threads = (hidden + 127) / 128 * 32;
+  while (p.chunk < 64 && n * threads > p.chunk * 512 * 256) p.chunk *= 2;
   p.chunks = (n + p.chunk - 1) / p.chunk;
   auto take = [&](size_t bytes) {
     const size_t at = p.bytes;

@@ -50,39 +50,38 @@ def _run(grads, max_norm, norm_type, eps, out):
         raise ValueError(f"norm_type must be 1, 2 or inf, got {norm_type}")
     if not grads:
         return torch.zeros(())
-    dev = grads[0].device
-    if dev.type != "cuda":
+    index = grads[0].get_device()
+    if index < 0:
         raise ValueError("gradients must be on a CUDA device")
     lists = [grads] if out is None or out is grads else [grads, out]
+    types = []
     for group in lists:
-        for t in group:
-            if t.dtype not in _DTYPES:
-                raise ValueError(f"gradients must be float32, bfloat16 or float16, got {t.dtype}")
-            if t.device != dev:
-                raise ValueError(f"gradients on more than one device ({dev} and {t.device})")
-            if not _dense(t):
-                raise ValueError("gradients must be dense in memory (no gaps between elements)")
+        if any(t.get_device() != index for t in group):
+            raise ValueError("gradients on more than one device")
+        try:
+            types.append(array("i", [_DTYPES[t.dtype] for t in group]))
+        except KeyError as e:
+            raise ValueError(f"gradients must be float32, bfloat16 or float16, got {e.args[0]}") from None
+        if not all(t.is_contiguous() or _dense(t) for t in group):
+            raise ValueError("gradients must be dense in memory (no gaps between elements)")
     if len(lists) == 2:
         if len(out) != len(grads):
             raise ValueError(f"out holds {len(out)} tensors, expected {len(grads)}")
-        for g, o in zip(grads, out):
-            if o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous())):
-                raise ValueError("out must have the gradients' shapes and strides")
+        if any(g.shape != o.shape or not (g.is_contiguous() and o.is_contiguous() or g.stride() == o.stride())
+               for g, o in zip(grads, out)):
+            raise ValueError("out must have the gradients' shapes and strides")
     ptrs = [array("q", [t.data_ptr() for t in g]) for g in lists]
     if out is not None and len(set(ptrs[-1])) != len(out):
         used = [t.data_ptr() for t in lists[-1] if t.numel()]
         if len(set(used)) != len(used):
             raise ValueError("the same gradient is listed twice")
-    types = [array("i", [_DTYPES[t.dtype] for t in g]) for g in lists]
     numel = array("q", [t.numel() for t in grads])
     nbytes = _workspace_bytes(len(grads))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    norm = torch.empty((), dtype=torch.float32, device=dev)
+    first = grads[0]
+    ws, norm = first.new_empty(nbytes, dtype=torch.uint8), first.new_empty((), dtype=torch.float32)
     at = lambda a: a.buffer_info()[0]  # noqa: E731
-    with N.device_guard(dev):
-        N.call("mib_clip_grad_norm", at(ptrs[0]), None if out is None else at(ptrs[-1]), at(numel), at(types[0]),
-               None if out is None else at(types[-1]), len(grads), mode, max_norm, eps, N.ptr(norm), N.ptr(ws), nbytes,
-               N.stream_ptr(dev))
+    N.launch("mib_clip_grad_norm", index, at(ptrs[0]), None if out is None else at(ptrs[-1]), at(numel), at(types[0]),
+             None if out is None else at(types[-1]), len(grads), mode, max_norm, eps, norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 

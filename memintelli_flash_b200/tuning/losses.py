@@ -33,102 +33,108 @@ PreferenceLoss = namedtuple("PreferenceLoss", "loss chosen_rewards rejected_rewa
 
 def _layout(t):
     """Row addressing of a (..., V) tensor with unit column stride in at most two levels, or None."""
-    dims = [(n, s) for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    shape, strides = t.shape, t.stride()
+    cols = shape[-1]
+    if t.is_contiguous():
+        return N.OutLayout(max(1, t.numel() // cols), 0, cols, 1)
     merged = []
-    for n, s in reversed(dims):
+    for n, s in zip(reversed(shape[:-1]), reversed(strides[:-1])):
+        if n == 1:
+            continue
         if merged and s == merged[-1][0] * merged[-1][1]:
             merged[-1] = (merged[-1][0] * n, merged[-1][1])
         else:
             merged.append((n, s))
-    if len(merged) > 2 or (t.shape[-1] != 1 and t.stride(-1) != 1):
+    if len(merged) > 2 or (cols != 1 and strides[-1] != 1):
         return None
-    n, s = merged[0] if merged else (1, t.shape[-1])
-    if n > 1 and s < t.shape[-1]:
+    n, s = merged[0] if merged else (1, cols)
+    if n > 1 and s < cols:
         return None
-    return N.OutLayout(n, merged[1][1] if len(merged) == 2 else 0, s, 1)
+    return N.OutLayout(max(1, n), merged[1][1] if len(merged) == 2 else 0, s, 1)
 
 
-def _ints(t, what, device):
-    if t.dtype not in _INTS:
+def _ints(t, what, index):
+    """(t, 1 if it is int64): dense, on CUDA device ``index``."""
+    wide = _INTS.get(t.dtype)
+    if wide is None:
         raise ValueError(f"{what} must be int32 or int64, got {t.dtype}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the logits on {device}")
-    return t if t.is_contiguous() else t.contiguous()
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, the logits on cuda:{index}")
+    return (t if t.is_contiguous() else t.contiguous()), wide
 
 
-def _floats(t, what, shape, device):
-    if tuple(t.shape) != tuple(shape):
+def _floats(t, what, shape, index):
+    if t.shape != shape:
         raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the logits on {device}")
+    if t.get_device() != index:
+        raise ValueError(f"{what} is on {t.device}, the logits on cuda:{index}")
+    if t.dtype is torch.float32 and t.is_contiguous():
+        return t
     return t.detach().to(torch.float32).contiguous()
 
 
 class _Rows:
     """The checked rows of one call: the native description and the tensors it points into."""
+    __slots__ = ("n", "sequences", "logits", "targets", "cu", "index", "spec")
 
     def __init__(self, logits, targets, temperature, ignore_index, cu_seqlens=None):
-        if not logits.is_cuda:
+        index = logits.get_device()
+        if index < 0:
             raise ValueError("logits must be on a CUDA device")
-        if logits.dtype not in _DTYPES:
+        dtype = _DTYPES.get(logits.dtype)
+        if dtype is None:
             raise ValueError(f"logits must be float32, bfloat16 or float16, got {logits.dtype}")
-        if logits.dim() < 1 or logits.shape[-1] < 1:
+        shape = logits.shape
+        if len(shape) < 1 or shape[-1] < 1:
             raise ValueError("logits must be (..., V) with V >= 1")
-        if targets.shape != logits.shape[:-1]:
-            raise ValueError(f"targets has shape {tuple(targets.shape)}, expected {tuple(logits.shape[:-1])}")
+        if targets.shape != shape[:-1]:
+            raise ValueError(f"targets has shape {tuple(targets.shape)}, expected {tuple(shape[:-1])}")
         if not 0.0 < temperature < 1e30:
             raise ValueError("temperature must be positive")
-        dev = logits.device
-        logits = logits.detach()
         layout = _layout(logits)
         if layout is None:
-            logits = logits.contiguous()
+            logits = logits.detach().contiguous()
             layout = _layout(logits)
-        targets = _ints(targets, "targets", dev)
-        self.n = targets.numel()
-        if layout.rows_per_group < 1:            # no rows
-            layout.rows_per_group = 1
+        targets, wide = _ints(targets, "targets", index)
+        n = targets.numel()
+        cu, cu_wide, sequences, per = None, 0, 0, 0
         if cu_seqlens is not None:
             if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
                 raise ValueError("cu_seqlens must hold the S + 1 row offsets of S sequences")
-            cu_seqlens = _ints(cu_seqlens, "cu_seqlens", dev)
-            self.sequences, per = cu_seqlens.numel() - 1, 0
-        elif targets.dim() > 1:
-            per = targets.shape[-1]
-            self.sequences = self.n // per if per else 0
-        else:
-            self.sequences, per = 0, 0
-        self.logits, self.targets, self.cu, self.device = logits, targets, cu_seqlens, dev
-        self.spec = N.TokenRows(logits.data_ptr(), targets.data_ptr(), None if cu_seqlens is None else cu_seqlens.data_ptr(),
-                                self.n, logits.shape[-1], layout, ignore_index, self.sequences, per, temperature,
-                                _DTYPES[logits.dtype], _INTS[targets.dtype],
-                                0 if cu_seqlens is None else _INTS[cu_seqlens.dtype], 0)
+            cu_seqlens, cu_wide = _ints(cu_seqlens, "cu_seqlens", index)
+            cu, sequences = cu_seqlens.data_ptr(), cu_seqlens.numel() - 1
+        elif len(shape) > 2:
+            per = shape[-2]
+            sequences = n // per if per else 0
+        self.n, self.sequences, self.index = n, sequences, index
+        self.logits, self.targets, self.cu = logits, targets, cu_seqlens
+        self.spec = N.TokenRows(logits.data_ptr(), targets.data_ptr(), cu, n, shape[-1], layout, ignore_index, sequences,
+                                per, temperature, dtype, wide, cu_wide, 0)
 
-    def workspace(self, sequences):
-        nbytes = _workspace_bytes(self.n, self.spec.cols, sequences)
-        return torch.empty(nbytes, dtype=torch.uint8, device=self.device), nbytes
+    def empty(self, shape):
+        return self.logits.new_empty(shape, dtype=torch.float32)
+
+    def workspace(self):
+        nbytes = _workspace_bytes(self.n, self.spec.cols, self.sequences)
+        return self.logits.new_empty(nbytes, dtype=torch.uint8), nbytes
 
     def gradient(self, out):
         """The gradient's tensor and row addressing."""
+        a = self.logits
         if out is None:
-            out = torch.empty(self.logits.shape, dtype=self.logits.dtype, device=self.device)
-        else:
-            if out.shape != self.logits.shape or out.dtype != self.logits.dtype or out.device != self.device:
-                raise ValueError("out must have the logits' shape, type and device")
-            if out.requires_grad and torch.is_grad_enabled():
-                raise ValueError("out must not require a gradient")
+            out = a.new_empty(a.shape)
+            return out, _layout(out)
+        if out.shape != a.shape or out.dtype != a.dtype or out.get_device() != self.index:
+            raise ValueError("out must have the logits' shape, type and device")
         layout = _layout(out)
-        rows = 0 if layout is None else layout.rows_per_group
-        if layout is None or (self.n > rows and layout.group_stride < (rows - 1) * layout.row_stride + out.shape[-1]):
+        if layout is None or (self.n > layout.rows_per_group and
+                              layout.group_stride < (layout.rows_per_group - 1) * layout.row_stride + out.shape[-1]):
             raise ValueError("out needs a unit column stride and rows that do not overlap")
-        a, b = self.logits, out
-        if a.data_ptr() == b.data_ptr():
-            if a.stride() != b.stride() and self.n > 1:
+        if a.data_ptr() == out.data_ptr():
+            if a.stride() != out.stride() and self.n > 1:
                 raise ValueError("out overlaps the logits without being the same rows")
-        elif a.numel() and _span(a)[0] < _span(b)[1] and _span(b)[0] < _span(a)[1]:
+        elif self.n and _span(a)[0] < _span(out)[1] and _span(out)[0] < _span(a)[1]:
             raise ValueError("out overlaps the logits without being the same rows")
-        if rows < 1:
-            layout.rows_per_group = 1
         return out, layout
 
 
@@ -136,6 +142,10 @@ def _span(t):
     """First byte and one past the last byte that a tensor reaches."""
     last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _address(t):
+    return None if t is None else t.data_ptr()
 
 
 @lru_cache(maxsize=256)
@@ -164,19 +174,16 @@ class TokenLogprobsRunc(torch.autograd.Function):
         rows = _Rows(logits, targets, *ctx.args)
         grad, layout = rows.gradient(None)
         if rows.n:
-            g = _floats(grad_logps, "the gradient", targets.shape, rows.device)
-            with N.device_guard(rows.device):
-                N.call("mib_token_logps_grad", rows.spec, N.ptr(stats), N.ptr(g), N.ptr(grad), layout,
-                       N.stream_ptr(rows.device))
+            g = _floats(grad_logps, "the gradient", targets.shape, rows.index)
+            N.launch("mib_token_logps_grad", rows.index, rows.spec, stats.data_ptr(), g.data_ptr(), grad.data_ptr(), layout)
         return grad, None, None, None
 
 
 def _token_logps(rows, keep_stats):
-    logps = torch.empty(rows.targets.shape, dtype=torch.float32, device=rows.device)
-    stats = torch.empty(rows.n, 4, dtype=torch.float32, device=rows.device) if keep_stats else None
+    logps = rows.empty(rows.targets.shape)
+    stats = rows.empty((rows.n, 4)) if keep_stats else None
     if rows.n:
-        with N.device_guard(rows.device):
-            N.call("mib_token_logps", rows.spec, N.ptr(logps), N.ptr(stats), N.stream_ptr(rows.device))
+        N.launch("mib_token_logps", rows.index, rows.spec, logps.data_ptr(), _address(stats))
     return logps, stats
 
 
@@ -191,8 +198,8 @@ def token_logprobs(logits, targets, *, temperature=1.0, ignore_index=-100):
 def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, reduction,
             temperature, ignore_index, want_grad, out):
     rows = _Rows(logits, targets, float(temperature), int(ignore_index), cu_seqlens)
-    dev = rows.device
-    if reduction not in _REDUCTIONS:
+    mode = _REDUCTIONS.get(reduction)
+    if mode is None:
         raise ValueError(f"reduction must be one of {sorted(_REDUCTIONS)}, got {reduction!r}")
     clip_high = clip_low if clip_high is None else clip_high
     if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < float("inf")):
@@ -201,27 +208,25 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_hi
         raise ValueError("kl_coef must be non-negative")
     if kl_coef > 0.0 and ref_logps is None:
         raise ValueError("the KL term needs ref_logps")
-    if reduction == "sequence" and rows.sequences < 1 and rows.n:
+    if mode == 1 and rows.sequences < 1 and rows.n:
         raise ValueError("the sequence mean needs a (B, T) batch or cu_seqlens")
-    shape = targets.shape
-    old = _floats(old_logps, "old_logps", shape, dev)
+    index, shape = rows.index, targets.shape
+    old = _floats(old_logps, "old_logps", shape, index)
     per_token = advantages.shape == shape
     if not per_token and (rows.sequences < 1 or advantages.numel() != rows.sequences):
         raise ValueError(f"advantages has shape {tuple(advantages.shape)}, expected {tuple(shape)} or one per sequence "
                          f"({rows.sequences})")
-    adv = _floats(advantages, "advantages", shape if per_token else advantages.shape, dev)
-    ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, dev)
+    adv = _floats(advantages, "advantages", advantages.shape, index)
+    ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, index)
     grad, layout = rows.gradient(out) if want_grad else (None, None)
+    logps, res = rows.empty(shape), rows.empty(3)
     if rows.n == 0:
-        z = torch.zeros(3, dtype=torch.float32, device=dev)
-        return PolicyLoss(z[0], torch.zeros(shape, dtype=torch.float32, device=dev), z[1], z[2]), grad
-    logps = torch.empty(shape, dtype=torch.float32, device=dev)
-    res = torch.empty(3, dtype=torch.float32, device=dev)
-    ws, nbytes = rows.workspace(rows.sequences)
-    spec = N.PolicySpec(clip_low, clip_high, kl_coef, _REDUCTIONS[reduction], 0 if per_token else 1)
-    with N.device_guard(dev):
-        N.call("mib_policy_loss", rows.spec, spec, N.ptr(old), N.ptr(adv), N.ptr(ref), N.ptr(res), N.ptr(logps),
-               N.ptr(grad), layout, N.ptr(ws), nbytes, N.stream_ptr(dev))
+        res.zero_()
+    else:
+        ws, nbytes = rows.workspace()
+        spec = N.PolicySpec(clip_low, clip_high, kl_coef, mode, 0 if per_token else 1)
+        N.launch("mib_policy_loss", index, rows.spec, spec, old.data_ptr(), adv.data_ptr(), _address(ref), res.data_ptr(),
+                 logps.data_ptr(), _address(grad), layout, ws.data_ptr(), nbytes)
     loss, kl, clipped = res.unbind(0)
     return PolicyLoss(loss, logps, kl, clipped), grad
 
@@ -244,9 +249,7 @@ class _LossRunc(torch.autograd.Function):
                                "forward pass")
         if grad.numel():
             factor = grad_loss.to(torch.float32).contiguous()
-            with N.device_guard(grad.device):
-                N.call("mib_scale_by", N.ptr(grad), _DTYPES[grad.dtype], grad.numel(), N.ptr(factor),
-                       N.stream_ptr(grad.device))
+            N.launch("mib_scale_by", grad.get_device(), grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), factor.data_ptr())
         return grad, None
 
 
@@ -278,10 +281,10 @@ def policy_loss_grad(logits, targets, old_logps, advantages, ref_logps=None, *, 
 def _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, margin, kind, average, temperature,
                 ignore_index, want_grad, out):
     rows = _Rows(logits, targets, float(temperature), int(ignore_index), cu_seqlens)
-    dev = rows.device
-    if kind not in _KINDS:
+    mode = _KINDS.get(kind)
+    if mode is None:
         raise ValueError(f"kind must be one of {sorted(_KINDS)}, got {kind!r}")
-    if not 0.0 <= label_smoothing <= 0.5 or (kind != "sigmoid" and label_smoothing):
+    if not 0.0 <= label_smoothing <= 0.5 or (mode != 0 and label_smoothing):
         raise ValueError("label_smoothing must be in [0, 0.5], and 0 except for the sigmoid loss")
     if not 0.0 < beta < 1e30:
         raise ValueError("beta must be positive")
@@ -290,19 +293,16 @@ def _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, m
     if rows.sequences < 2 or rows.sequences % 2:
         raise ValueError("preference pairs need an even number of sequences: the chosen ones, then the rejected ones "
                          f"in the same order (got {rows.sequences})")
-    shape, pairs = targets.shape, rows.sequences // 2
-    ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, dev)
-    grad, layout = rows.gradient(out) if want_grad else (None, None)
-    logps = torch.empty(shape, dtype=torch.float32, device=dev)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    chosen, rejected = (torch.empty(pairs, dtype=torch.float32, device=dev) for _ in range(2))
     if rows.n == 0:
         raise ValueError("preference pairs need rows")
-    ws, nbytes = rows.workspace(rows.sequences)
-    spec = N.PreferenceSpec(beta, label_smoothing, margin, _KINDS[kind], 1 if average else 0)
-    with N.device_guard(dev):
-        N.call("mib_preference_loss", rows.spec, spec, N.ptr(ref), N.ptr(loss), N.ptr(chosen), N.ptr(rejected),
-               N.ptr(logps), N.ptr(grad), layout, N.ptr(ws), nbytes, N.stream_ptr(dev))
+    index, shape, pairs = rows.index, targets.shape, rows.sequences // 2
+    ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, index)
+    grad, layout = rows.gradient(out) if want_grad else (None, None)
+    logps, loss, chosen, rejected = rows.empty(shape), rows.empty(()), rows.empty(pairs), rows.empty(pairs)
+    ws, nbytes = rows.workspace()
+    spec = N.PreferenceSpec(beta, label_smoothing, margin, mode, 1 if average else 0)
+    N.launch("mib_preference_loss", index, rows.spec, spec, _address(ref), loss.data_ptr(), chosen.data_ptr(),
+             rejected.data_ptr(), logps.data_ptr(), _address(grad), layout, ws.data_ptr(), nbytes)
     return PreferenceLoss(loss, chosen, rejected, logps), grad
 
 
