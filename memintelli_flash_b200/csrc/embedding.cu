@@ -69,6 +69,7 @@ cudaError_t lookup_words(IntList ids, int64_t n, const void* table, int64_t voca
                          float scale, void* out, cudaStream_t stream) {
   const int64_t words = hidden * static_cast<int64_t>(sizeof(T)) / BYTES;
   const int64_t chunks = (words + 127) / 128;
+  if (chunks > (int64_t(1) << 33) / n) return cudaErrorInvalidValue;
   lookup_kernel<T, BYTES><<<static_cast<unsigned>((n * chunks + 7) / 8), 256, 0, stream>>>(
       ids, n, static_cast<const T*>(table), vocab, hidden, ld, scale, static_cast<T*>(out), static_cast<int>(chunks));
   count_launch();
@@ -661,8 +662,8 @@ cudaError_t embed_grad_t(EmbedGradArgs a, SortArgs s, void* workspace, cudaStrea
   }
   if (e == cudaSuccess && !a.accumulate) {
     const ZeroArgs z{a.out, a.vocab, a.hidden * static_cast<int64_t>(sizeof(O)), a.ld_out * static_cast<int64_t>(sizeof(O))};
-    const int64_t want = (z.rows * z.row_bytes + 32767) / 32768;  // 4 vectors a thread, up to 4 blocks an SM
-    e = launch_kernel(zero_kernel, want < 148 * 4 ? want : 148 * 4, 512, 1, true, z, stream);
+    const int64_t want = (z.rows * z.row_bytes + 32767) / 32768;  // 4 vectors a thread
+    e = launch_kernel(zero_kernel, want < (1 << 20) ? want : (1 << 20), 512, 1, true, z, stream);
   }
   if (e != cudaSuccess) return e;
   constexpr int V = kVec16<G>;

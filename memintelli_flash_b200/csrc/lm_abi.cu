@@ -77,7 +77,8 @@ TokenSpace token_space(int64_t rows, int64_t sequences) {
   return s;
 }
 
-mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
+// `both`: log2(e) / T in two numbers (the losses).
+mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row, bool both) {
   mib::TokenArgs a{};
   a.logits = t->logits;
   a.map = row_map(t->layout);
@@ -85,9 +86,18 @@ mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
   a.cols = t->cols;
   a.targets = mib::IntList{t->targets, t->targets_i64};
   a.ignore_index = t->ignore_index;
-  a.k = static_cast<float>(1.4426950408889634 / t->temperature);
+  const double k = 1.4426950408889634 / t->temperature;
+  a.k.hi = static_cast<float>(k);
+  a.k.lo = mib::kNoLow;
+  a.k.inv_hi = static_cast<float>(1.0 / t->temperature);
+  if (static_cast<double>(a.k.inv_hi) >= 1.0 / t->temperature) a.k.inv_hi = std::nextafter(a.k.inv_hi, 0.0f);
+  a.k.inv_lo = static_cast<float>(1.0 / t->temperature - static_cast<double>(a.k.inv_hi));
+  if (both) {
+    if (static_cast<double>(a.k.hi) >= k) a.k.hi = std::nextafter(a.k.hi, 0.0f);
+    a.k.lo = static_cast<float>(k - static_cast<double>(a.k.hi));
+  }
+  a.inv_temp_k = (static_cast<double>(a.k.hi) + (both ? static_cast<double>(a.k.lo) : 0.0)) * 0.6931471805599453;
   a.inv_temp = 1.0 / t->temperature;
-  a.inv_temp_k = static_cast<double>(a.k) * 0.6931471805599453;
   a.logps = logps;
   a.row = static_cast<float4*>(row);
   return a;
@@ -136,7 +146,7 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
     return fail(MIB_ERR_UNSUPPORTED, "gradients are fp32, bf16 or fp16; the table's gradient has that type or fp32");
   if (n < 1 || vocab < 1 || hidden < 1 || ld_grad < hidden || ld_out < hidden)
     return fail(MIB_ERR_SHAPE, "invalid embedding shape");
-  if (n >= kMaxRows || vocab >= kMaxRows || hidden > (1 << 24)) return fail(MIB_ERR_SHAPE, "too many tokens, rows or columns");
+  if (n >= kMaxRows || vocab >= kMaxRows || hidden > (1 << 23)) return fail(MIB_ERR_SHAPE, "too many tokens, rows or columns");
   if (int r = check_space(workspace, workspace_bytes, static_cast<int64_t>(mib::embed_plan(n, vocab, hidden).bytes))) return r;
   mib::EmbedGradArgs a{};
   a.n = n;
@@ -173,7 +183,7 @@ int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, cudaStre
   if (int r = check_token_rows(t)) return r;
   if (!logps || reinterpret_cast<uintptr_t>(stats) % 16) return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
   mib::RowArgs a{};
-  a.t = token_args(t, logps, stats);
+  a.t = token_args(t, logps, stats, false);
   cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::token_logps_t<decltype(v)>(a, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "token_logps launch");
   return MIB_OK;
@@ -186,7 +196,7 @@ int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float
     return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
   if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
   mib::GradArgs g{};
-  g.t = token_args(t, nullptr, const_cast<void*>(stats));
+  g.t = token_args(t, nullptr, const_cast<void*>(stats), false);
   g.slope = grad_logps;
   g.grad = grad;
   g.gmap = row_map(*grad_layout);
@@ -214,7 +224,7 @@ int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const 
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
   mib::RowArgs a{};
-  a.t = token_args(t, logps, nullptr);
+  a.t = token_args(t, logps, nullptr, true);
   a.seq = seq_list(t);
   a.old_logps = old_logps;
   a.advantages = advantages;
@@ -257,7 +267,7 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
   mib::RowArgs rows{};
-  rows.t = token_args(t, logps, grad ? ws + s.row : nullptr);
+  rows.t = token_args(t, logps, grad ? ws + s.row : nullptr, true);
   rows.seq = seq_list(t);
   rows.ref_logps = ref_logps;
   rows.done = reinterpret_cast<uint32_t*>(ws + s.done);

@@ -20,12 +20,31 @@ namespace mib {
 
 constexpr float kLowest = -3.402823466e38f;
 
+// log2(e) / T as hi + lo.  One fp32 number is up to 6e-8 off, which every exponential of a row has in the same direction:
+// nothing next to a log-probability's own rounding, but summed over a sequence's tokens more than all their roundings.
+// So the losses use both (one operation more per element), with hi rounded down and lo above zero: -inf times lo then is
+// -inf too.  Plain log-probabilities use hi alone (lo is kNoLow: 2048 x 151936 bf16 87 us; 92 us with both), with the
+// temperature that hi stands for.
+struct Scale {
+  float hi, lo;
+  float inv_hi, inv_lo;  // 1 / T likewise
+};
+constexpr float kNoLow = 1e-30f;
+__device__ __forceinline__ Scale hi_only(Scale k) {
+  k.lo = 0.0f;
+  return k;
+}
+// exp(d / T) for joining the threads' and warps' sums.  Not by ex2: its mean error would come on top at every join.
+__device__ __forceinline__ float exp_join(float d, Scale k) { return expf(fmaf(d, k.inv_hi, d * k.inv_lo)); }
+// exp(d / T) for elements
+__device__ __forceinline__ float exp_scaled(float d, Scale k) { return ex2(fmaf(d, k.hi, d * k.lo)); }
+
 struct RowStat {
   float m, s;
 };
-__device__ __forceinline__ RowStat merge(RowStat a, RowStat b, float k) {
+__device__ __forceinline__ RowStat merge(RowStat a, RowStat b, Scale k) {
   const float m = fmaxf(a.m, b.m);
-  return RowStat{m, a.s * ex2((a.m - m) * k) + b.s * ex2((b.m - m) * k)};
+  return RowStat{m, a.s * exp_join(a.m - m, k) + b.s * exp_join(b.m - m, k)};
 }
 
 // Elements in front of the first 16-byte boundary of a row at p (all of them when there is none).
@@ -65,37 +84,38 @@ __device__ __forceinline__ float vec_max(const uint4& u, float m) {
   }
 }
 
-// The reference of a set of exponentials 2^((v - m) k).  The fast form is 2^(v k - mk) in one fused operation, with mk
-// the rounded m k; `corr` (a relative correction of the results, at most 4e-4 with a square of 2e-7) makes up for that
+// The reference of a set of exponentials exp((v - m) / T).  The fast form is 2^(v k - mk) in fused operations, with mk the
+// rounded m k; `corr` (a relative correction of the results, at most 4e-4 with a square of 2e-7) makes up for that
 // rounding.  Where m k is larger (rows of a type's lowest value, say) v - m comes first: equal values give exactly 1.
 struct ExpRef {
   float m, mk, corr;
   bool fast;
-  __device__ __forceinline__ void set(float max, float k) {
+  __device__ __forceinline__ void set(float max, Scale k) {
     m = max;
-    mk = max * k;
-    corr = -0.6931472f * fmaf(max, k, -mk);
+    mk = max * k.hi;
+    corr = -0.6931472f * fmaf(max, k.lo, fmaf(max, k.hi, -mk));
     fast = fabsf(mk) < 8192.0f;
     if (!fast) corr = 0.0f;
   }
 };
 
-// The exponentials of a vector's elements (without the correction).
-template <typename T, bool FAST>
-__device__ __forceinline__ void vec_exp(const uint4& u, const ExpRef& r, float k, float (&v)[kVec16<T>]) {
-  unpack16<T>(u, v);
-#pragma unroll
-  for (int e = 0; e < kVec16<T>; ++e) v[e] = ex2(FAST ? fmaf(v[e], k, -r.mk) : (v[e] - r.m) * k);
-}
-
-// Their sum over N vectors, as a tree, corrected.
-template <typename T, bool FAST, int N>
-__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, float k) {
+// The sum of the exponentials of N vectors' elements, as trees, corrected.
+template <typename T, bool FAST, bool LOW, int N>
+__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, Scale k) {
   float s = 0.0f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float v[kVec16<T>];
-    vec_exp<T, FAST>(u[i], r, k, v);
+    unpack16<T>(u[i], v);
+#pragma unroll
+    for (int e = 0; e < kVec16<T>; ++e) {
+      if (FAST) {
+        const float y = fmaf(v[e], k.hi, -r.mk);
+        v[e] = ex2(LOW ? fmaf(v[e], k.lo, y) : y);
+      } else {
+        v[e] = exp_scaled(v[e] - r.m, k);
+      }
+    }
 #pragma unroll
     for (int w = kVec16<T> / 2; w > 0; w >>= 1)
 #pragma unroll
@@ -105,31 +125,33 @@ __device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, 
   return fmaf(s, r.corr, s);
 }
 template <typename T, int N>
-__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, float k) {
-  return r.fast ? vecs_sum<T, true>(u, r, k) : vecs_sum<T, false>(u, r, k);
+__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, Scale k) {
+  if (!r.fast) return vecs_sum<T, false, true>(u, r, k);
+  return k.lo > kNoLow ? vecs_sum<T, true, true>(u, r, k) : vecs_sum<T, true, false>(u, r, k);
 }
 
-// N vectors of logits to q times their exponentials, in the logits' type.
+// N vectors of logits to q times their exponentials, in the logits' type.  Here k.hi is enough (the reference is set with
+// it alone): a gradient element's relative error of 1e-7 stays its own.
 template <typename T, bool FAST, int N>
-__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, float k, float q) {
+__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, Scale k, float q) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float v[kVec16<T>];
-    vec_exp<T, FAST>(u[i], r, k, v);
+    unpack16<T>(u[i], v);
 #pragma unroll
-    for (int e = 0; e < kVec16<T>; ++e) v[e] *= q;
+    for (int e = 0; e < kVec16<T>; ++e) v[e] = q * ex2(FAST ? fmaf(v[e], k.hi, -r.mk) : (v[e] - r.m) * k.hi);
     u[i] = pack16<T>(v);
   }
 }
 template <typename T, int N>
-__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, float k, float q) {
+__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, Scale k, float q) {
   if (r.fast) vecs_grad<T, true>(u, r, k, q);
   else vecs_grad<T, false>(u, r, k, q);
 }
 
-// Mean relative error of ex2.approx over its argument's fractions, measured on a B200 (2^20 arguments in [-24, 0]).
-// A sum of many exponentials carries it; summed over a sequence's tokens it would outgrow the rounding errors.
-constexpr float kEx2Mean = -5.2e-8f;
+// Mean relative error of a softmax's sum of ex2.approx results, measured on a B200 as the mean error of log-probabilities
+// against 64 bits (vocabularies of 500 to 151936, three types, two temperatures).  A sequence's tokens would add it up.
+constexpr float kEx2Mean = -2.5e-8f;
 
 // log s for s in (0, 2^127]: exponent and mantissa apart, so that the error is that of the log of a number near 1
 // (3e-8) and not half an ulp of the result (5e-7 for a vocabulary's sum).  0 gives -inf, NaN and inf themselves.
@@ -146,9 +168,9 @@ struct TokenArgs {
   int64_t rows, cols;
   IntList targets;
   int64_t ignore_index;
-  float k;             // log2(e) / T, rounded
+  Scale k;             // log2(e) / T
   double inv_temp;     // 1 / T
-  double inv_temp_k;   // k log(2): 1 / T as k has it, which the target's logit takes like the others
+  double inv_temp_k;   // k log(2), which the target's logit takes like the others
   float* logps;        // [rows]
   float4* row;         // [rows] {m, 1 / s, c, -}, or null
 };
@@ -309,11 +331,11 @@ __device__ __forceinline__ void cluster_store(RowStat* p, uint32_t rank, RowStat
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(v.m), "f"(v.s) : "memory");
 }
 
-__device__ __forceinline__ RowStat warp_merge(RowStat t, float k) {
+__device__ __forceinline__ RowStat warp_merge(RowStat t, Scale k) {
   float m = t.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float s = t.s * ex2((t.m - m) * k);
+  float s = t.s * exp_join(t.m - m, k);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   return RowStat{m, s};
@@ -409,7 +431,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) st.m = fmaxf(st.m, __shfl_xor_sync(0xffffffffu, st.m, o));
       ref.set(st.m, a.t.k);
-      st.s = vecs_sum<T>(v, ref, a.t.k) + ex2((edge - st.m) * a.t.k);
+      st.s = vecs_sum<T>(v, ref, a.t.k) + exp_scaled(edge - st.m, a.t.k);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
     } else {
@@ -421,11 +443,11 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 #pragma unroll
         for (int u = 0; u < NV; ++u) m = vec_max<T>(v[u], m);
         ref.set(m, a.t.k);
-        st.s = fmaf(st.s, ex2((st.m - m) * a.t.k), vecs_sum<T>(v, ref, a.t.k));
+        st.s = fmaf(st.s, exp_scaled(st.m - m, a.t.k), vecs_sum<T>(v, ref, a.t.k));
         st.m = m;
       }
       const float m = fmaxf(edge, st.m);
-      st.s = st.s * ex2((st.m - m) * a.t.k) + ex2((edge - m) * a.t.k);
+      st.s = st.s * exp_join(st.m - m, a.t.k) + exp_scaled(edge - m, a.t.k);
       st.m = m;
       st = warp_merge(st, a.t.k);
     }
@@ -480,7 +502,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
     if (a.grad && have) {
       T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
       const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-      ref.set(st.m, a.t.k);
+      ref.set(st.m, hi_only(a.t.k));
       const float q0 = -coef / st.s, q = fmaf(q0, ref.corr, q0);
       const bool zero = coef == 0.0f;  // zeros whatever the logits hold, NaN and infinities included
       const bool hit = t >= 0 && t < cols;
@@ -514,11 +536,11 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
           store(i);
         }
       }
-      if (edge_at >= 0) g[edge_at] = from_f32<T>(zero ? 0.0f : q0 * ex2((edge - st.m) * a.t.k));
+      if (edge_at >= 0) g[edge_at] = from_f32<T>(zero ? 0.0f : q0 * exp_scaled(edge - st.m, a.t.k));
       if (hit && !zero) {  // the target's element again, by the thread that wrote it
         const int j = static_cast<int>(t), i = (j - head) / V;
         if (j == edge_at || (j >= head && i < nvec && i >= begin && i < begin + per && (i - begin) % GROUP == tid))
-          g[j] = from_f32<T>(fmaf(q0, ex2((target_logit - st.m) * a.t.k), coef));
+          g[j] = from_f32<T>(fmaf(q0, exp_scaled(target_logit - st.m, a.t.k), coef));
       }
     }
     __syncthreads();
@@ -741,7 +763,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
   } else {  // ---- arithmetic
     const int tid = threadIdx.x;
     const uint32_t none = neg_inf_word<T>();
-    const float k2 = a.t.k;
+    const Scale k2 = a.t.k;
     RingPos<SLOTS> pos;
     int64_t live = 0;
     bool ok = true;
@@ -788,15 +810,17 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
 #pragma unroll
           for (int u = 0; u < VECS; ++u) v[u] = u * CT < left ? base[u * CT] : make_uint4(none, none, none, none);
         }
-        float m = st.m;
-#pragma unroll
-        for (int u = 0; u < VECS; ++u) m = vec_max<T>(v[u], m);
         if (c < n - keep) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty[pos.slot]);
         }
+        // The reference follows the thread's maximum: the largest exponentials, which carry the row, are exact or nearly
+        // (a reference kept from the first part saves 5% and makes the log-probability's error three times as large).
+        float m = st.m;
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) m = vec_max<T>(v[u], m);
         if (m > st.m) {
-          st.s *= ex2((st.m - m) * k2);
+          st.s *= exp_scaled(st.m - m, k2);
           st.m = m;
           ref.set(m, k2);
         }
@@ -804,7 +828,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         pos.next();
       }
       const float m = fmaxf(edge, st.m);
-      st.s = st.s * ex2((st.m - m) * k2) + ex2((edge - m) * k2);
+      st.s = st.s * exp_join(st.m - m, k2) + exp_scaled(edge - m, k2);
       st.m = m;
       st = warp_merge(st, k2);
       const int h = static_cast<int>(live & 1);
@@ -822,7 +846,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
       ok = __all_sync(0xffffffffu, mbar_wait(&coef_full, static_cast<uint32_t>(live - 1) & 1, &abort_flag, kErr + 9));
       if (!ok) break;
       const float4 f = row_coef;
-      ref.set(f.x, k2);
+      ref.set(f.x, hi_only(k2));
       const float coef = f.y, q0 = f.z, q = fmaf(q0, ref.corr, q0);
       T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
       uint4* gv = reinterpret_cast<uint4*>(g + head) + tid;
@@ -860,12 +884,12 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         }
       }
       if (n > keep) pos = at;
-      if (edge_at >= 0) g[edge_at] = from_f32<T>(q0 * ex2((edge - f.x) * k2));
+      if (edge_at >= 0) g[edge_at] = from_f32<T>(q0 * exp_scaled(edge - f.x, k2));
       // the target's element again, by the thread that wrote it
       if (t >= 0 && t < cols) {
         const int j = static_cast<int>(t), i = (j - head) / V;
         if (j == edge_at || (j >= head && i < nvec && i % CT == tid))
-          g[j] = from_f32<T>(fmaf(q0, ex2((f.w - f.x) * k2), coef));
+          g[j] = from_f32<T>(fmaf(q0, exp_scaled(f.w - f.x, k2), coef));
       }
     }
   }
@@ -984,11 +1008,11 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
   T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
   ExpRef ref;
-  ref.set(st.x, a.t.k);
+  ref.set(st.x, hi_only(a.t.k));
   const float q0 = -c * st.y, q = fmaf(q0, ref.corr, q0);
   const bool zero = c == 0.0f;
   float at_t = 0.0f;
-  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q0, ex2((to_f32(p[t]) - st.x) * a.t.k), c);
+  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q0, exp_scaled(to_f32(p[t]) - st.x, a.t.k), c);
   if (p == g) __syncthreads();
   const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   const int64_t head = same ? peel(g, a.t.cols) : a.t.cols;
@@ -1014,7 +1038,7 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
       if (i0 + u * 256 < end) __stcs(gv + i0 + u * 256, raw[u]);
   }
   auto one = [&](int64_t j) {
-    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q0 * ex2((to_f32(p[j]) - st.x) * a.t.k)));
+    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q0 * exp_scaled(to_f32(p[j]) - st.x, a.t.k)));
   };
   // the target's element again, by the thread that wrote it
   if (!zero && tv >= per * part && tv < end && (tv - per * part) % 256 == threadIdx.x) g[t] = from_f32<T>(at_t);

@@ -334,3 +334,59 @@ def test_refusals_on_device_tensors(cuda):
         with pytest.raises(ValueError):
             f()
             pytest.fail(f"refusal {i} did not happen")
+
+
+def test_rising_logits_in_long_rows(cuda):
+    """Later parts of a row far above its first ones: the running reference has to follow, by a little or by a lot."""
+    for dtype in DTYPES:
+        for step in (0.5, 30.0, 200.0, 20000.0):
+            x, t, _ = make(200, 40000, dtype, 11, spread=1.0)
+            x = (x.float() + (torch.arange(40000, device="cuda") // 5000) * step).to(dtype)
+            t[:] = torch.randint(39000, 40000, (200,), device="cuda")
+            x[1, :39000] = -math.inf
+            x[2, :39000] = torch.finfo(dtype).min
+            x[3, 39999], t[3] = math.nan, 5
+            want, p = O.row_logps(x, t)
+            old = want.nan_to_num(0.0).float().cuda()
+            near_logps(tuning.token_logprobs(x, t), want)
+            r, grad = tuning.policy_loss_grad(x, t, old, torch.ones(200, device="cuda"), reduction="sum")
+            near_logps(r.logps, want)
+            rows = [i for i in range(200) if i != 3]
+            slope = -torch.exp(want - old.double().cpu())[rows]
+            near_grad(grad[rows], O.logit_grad(p[rows], t[rows], slope), dtype, more=2e-5)
+            assert grad[3].isnan().all()
+
+
+def test_rows_past_32_bit_offsets(cuda):
+    """More than 2^31 logits: the last rows are where 32-bit offsets would have wrapped."""
+    n, v = 16500, 131072
+    x = torch.zeros(n, v, dtype=torch.bfloat16, device="cuda")
+    rows = torch.tensor([0, 1, n - 2, n - 1], device="cuda")
+    x[rows] = (torch.randn(4, v, device="cuda") * 2).bfloat16()
+    t = torch.full((n,), O.IGNORE, device="cuda")
+    t[rows] = torch.tensor([5, v - 1, 0, v - 1], device="cuda")
+    want, p = O.row_logps(x[rows], t[rows])
+    near_logps(tuning.token_logprobs(x, t)[rows], want)
+    old = torch.zeros(n, device="cuda")
+    old[rows] = want.float().cuda()
+    r, grad = tuning.policy_loss_grad(x, t, old, torch.ones(n, device="cuda"), reduction="sum", out=x)
+    near(r.loss, torch.tensor(-4.0), 1e-4)
+    near_grad(grad[rows], O.logit_grad(p, t[rows], -torch.ones(4, dtype=torch.float64)), torch.bfloat16, more=2e-5)
+
+
+def test_losses_in_a_cuda_graph(cuda):
+    cu = [0, 100, 333]
+    x, t, old, adv, ref = policy_inputs(333, 5003, torch.bfloat16, 8, cu, True)
+    y = policy_inputs(333, 5003, torch.bfloat16, 9, cu, True)[0]
+    kw = dict(cu_seqlens=torch.tensor(cu, device="cuda"))
+    run = lambda: (tuning.policy_loss_grad(x, t, old, adv, ref, **kw), tuning.preference_loss_grad(x, t, ref, **kw),  # noqa: E731
+                   tuning.token_logprobs(x, t))
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        (a, ga), (p, gp), lp = run()
+    x.copy_(y)
+    graph.replay()
+    (b, gb), (q, gq), lq = run()
+    assert all(torch.equal(u, v) for u, v in zip((*a, ga, *p, gp, lp), (*b, gb, *q, gq, lq)))

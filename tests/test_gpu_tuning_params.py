@@ -157,6 +157,37 @@ def test_embedding_module_and_differences(cuda):
     assert abs(diff / 2 - (m.weight.grad * d).sum().item()) <= 4e-6 * size
 
 
+def test_tables_past_32_bit_offsets(cuda):
+    vocab, hidden = 530000, 4100
+    w = torch.zeros(vocab, hidden, dtype=torch.bfloat16, device="cuda")
+    w[-3:] = torch.randn(3, hidden, device="cuda").bfloat16()
+    ids = torch.tensor([vocab - 1, 0, vocab - 3, vocab - 2, vocab - 1], device="cuda")
+    assert torch.equal(embedding_scaled(ids, w), w[ids])
+    g = torch.randn(5, hidden, device="cuda").bfloat16()
+    out = embedding_scaled_grad(ids, g, vocab, out=w)
+    check = torch.stack([g[1], g[2], g[3], (g[0].float() + g[4].float()).bfloat16()])
+    assert torch.equal(out[[0, vocab - 3, vocab - 2, vocab - 1]], check)
+    assert not out[1:vocab - 3].any()
+
+
+def test_parameter_operators_in_a_cuda_graph(cuda):
+    ids = torch.randint(0, 500, (700,), device="cuda")
+    g = torch.randn(700, 96, device="cuda")
+    grads = make_grads([5000, 17, 300000], [torch.float32, torch.bfloat16], 2)
+    outs = [torch.empty_like(x) for x in grads]
+    run = lambda: (embedding_scaled_grad(ids, g, 500), tuning.clip_grad_norm_(grads, 0.5, out=outs))  # noqa: E731
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = run()
+    ids.copy_(torch.randint(0, 500, (700,), device="cuda"))
+    graph.replay()
+    kept = [x.clone() for x in outs]
+    b = run()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and all(torch.equal(x, y) for x, y in zip(kept, outs))
+
+
 # ---- clipping ------------------------------------------------------------------------------------------
 def make_grads(sizes, dtypes, seed, scale=0.05):
     g = gen(seed)
@@ -237,6 +268,15 @@ def test_clip_non_finite(cuda):
             want = math.nan if math.isnan(bad) else 0.0                         # 1 / inf; inf * 0 is NaN
             assert torch.equal(g[1].isnan(), torch.full((7,), math.isnan(want), device="cuda"))
             assert g[0][where].isnan()
+
+
+def test_clip_past_32_bit_offsets(cuda):
+    g = torch.zeros((1 << 31) + 1003, dtype=torch.bfloat16, device="cuda")
+    g[-5:], g[3] = 3.0, 4.0
+    norm = tuning.clip_grad_norm_([g[:7], g[7:]], 0.5).item()
+    assert norm == pytest.approx((5 * 9 + 16) ** 0.5, rel=5e-6)
+    want = torch.tensor(3.0 * 0.5 / (norm + 1e-6)).bfloat16().item()
+    assert g[-5:].tolist() == [want] * 5 and not g[100:-5].any()
 
 
 def test_clip_same_bits_twice(cuda):
