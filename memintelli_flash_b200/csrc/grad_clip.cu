@@ -4,7 +4,7 @@
 // launch.  Both passes walk fixed-size chunks; the norm's partial sums, one per block, are added in a fixed order, by
 // every block of the second pass for itself (at most 9.5 KB from L2, and one launch less).  The second pass walks the
 // chunks backwards: what the first read last is still in L2.  Both are bound by memory: 3 GB of fp32 gradients are read
-// at 6.9 TB/s, then scaled at 6.4 TB/s.
+// at 6.8 TB/s (440 us), then scaled at 6.3 TB/s (957 us).
 #include "kernels.cuh"
 #include "lm_common.cuh"
 

@@ -18,6 +18,9 @@ bool known_dtype(int32_t d) { return d == MIB_F32 || d == MIB_BF16 || d == MIB_F
 size_t dtype_size(int32_t d) { return d == MIB_F32 ? 4 : 2; }
 int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 
+bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+size_t index_size(int32_t is64) { return is64 ? 8 : 4; }
+
 // Calls fn with a value of the element type.
 template <typename F>
 cudaError_t with_dtype(int32_t d, F fn) {
@@ -30,9 +33,14 @@ constexpr int64_t kMaxRows = int64_t(1) << 31;
 
 mib::RowMap row_map(const mib_out_layout& l) { return mib::RowMap{l.rows_per_group, l.group_stride, l.row_stride}; }
 
+int check_grad(const mib_token_rows* t, const void* grad) {
+  return aligned(grad, dtype_size(t->dtype)) ? MIB_OK : fail(MIB_ERR_PARAM, "misaligned gradient");
+}
+
 int check_rows_layout(const mib_out_layout* l, int64_t rows, int64_t cols, const char* what) {
   if (!l) return fail(MIB_ERR_PARAM, std::string(what) + " layout is NULL");
-  if (l->rows_per_group < 1 || l->col_stride != 1) return fail(MIB_ERR_SHAPE, std::string(what) + " needs unit column stride and rows in groups");
+  if (l->rows_per_group < 1 || l->col_stride != 1) 
+    return fail(MIB_ERR_SHAPE, std::string(what) + " needs unit column stride and rows in groups");
   if (rows > 1 && l->rows_per_group > 1 && l->row_stride < cols)
     return fail(MIB_ERR_SHAPE, std::string(what) + " rows overlap");
   return MIB_OK;
@@ -44,7 +52,9 @@ int check_token_rows(const mib_token_rows* t) {
   if (t->rows < 1 || t->cols < 1) return fail(MIB_ERR_SHAPE, "logits must be non-empty");
   if (t->rows >= kMaxRows / 1024 || t->cols >= kMaxRows) return fail(MIB_ERR_SHAPE, "too many rows or columns");
   if (!(t->temperature > 0.0) || !(t->temperature < 1e30)) return fail(MIB_ERR_PARAM, "temperature must be positive");
-  if (reinterpret_cast<uintptr_t>(t->logits) % dtype_size(t->dtype)) return fail(MIB_ERR_PARAM, "misaligned logits");
+  if (!aligned(t->logits, dtype_size(t->dtype)) || !aligned(t->targets, index_size(t->targets_i64)) ||
+      !aligned(t->cu_seqlens, index_size(t->cu_i64)))
+    return fail(MIB_ERR_PARAM, "misaligned logits, targets or row offsets");
   return check_rows_layout(&t->layout, t->rows, t->cols, "logits");
 }
 
@@ -123,6 +133,8 @@ int mib_embedding_lookup(const void* ids, int32_t ids_i64, int64_t n, const void
   if (!known_dtype(dtype)) return fail(MIB_ERR_UNSUPPORTED, "the table must be fp32, bf16 or fp16");
   if (n < 1 || vocab < 1 || hidden < 1 || ld_table < hidden) return fail(MIB_ERR_SHAPE, "invalid embedding shape");
   if (n >= kMaxRows || hidden > (1 << 24)) return fail(MIB_ERR_SHAPE, "too many tokens or columns");
+  if (!aligned(ids, index_size(ids_i64)) || !aligned(table, dtype_size(dtype)) || !aligned(out, dtype_size(dtype)))
+    return fail(MIB_ERR_PARAM, "misaligned buffer");
   cudaError_t e = with_dtype(dtype, [&](auto v) {
     return mib::lookup_t<decltype(v)>(mib::IntList{ids, ids_i64}, n, table, vocab, hidden, ld_table, scale, out, stream);
   });
@@ -147,6 +159,8 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
   if (n < 1 || vocab < 1 || hidden < 1 || ld_grad < hidden || ld_out < hidden)
     return fail(MIB_ERR_SHAPE, "invalid embedding shape");
   if (n >= kMaxRows || vocab >= kMaxRows || hidden > (1 << 23)) return fail(MIB_ERR_SHAPE, "too many tokens, rows or columns");
+  if (!aligned(ids, index_size(ids_i64)) || !aligned(grad, dtype_size(grad_dtype)) || !aligned(out, dtype_size(out_dtype)))
+    return fail(MIB_ERR_PARAM, "misaligned buffer");
   if (int r = check_space(workspace, workspace_bytes, static_cast<int64_t>(mib::embed_plan(n, vocab, hidden).bytes))) return r;
   mib::EmbedGradArgs a{};
   a.n = n;
@@ -195,6 +209,7 @@ int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float
   if (!stats || !grad_logps || !grad || reinterpret_cast<uintptr_t>(stats) % 16)
     return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
   if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+  if (int r = check_grad(t, grad)) return r;
   mib::GradArgs g{};
   g.t = token_args(t, nullptr, const_cast<void*>(stats), false);
   g.slope = grad_logps;
@@ -218,8 +233,10 @@ int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const 
   if (spec->reduction < 0 || spec->reduction > 2) return fail(MIB_ERR_PARAM, "unknown reduction");
   if ((spec->reduction == 1 || spec->adv_per_sequence) && t->sequences < 1)
     return fail(MIB_ERR_PARAM, "a sequence mean or advantages per sequence need the sequences");
-  if (grad)
+  if (grad) {
     if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+    if (int r = check_grad(t, grad)) return r;
+  }
   const TokenSpace s = token_space(t->rows, t->sequences);
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
@@ -261,8 +278,10 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
     return fail(MIB_ERR_PARAM, "label smoothing must be in [0, 0.5], and 0 except for the sigmoid loss");
   if (!(spec->beta > 0.0) || !(spec->beta < 1e30) || !(std::fabs(spec->margin) < 1e30))
     return fail(MIB_ERR_PARAM, "beta must be positive and the margin finite");
-  if (grad)
+  if (grad) {
     if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+    if (int r = check_grad(t, grad)) return r;
+  }
   const TokenSpace s = token_space(t->rows, t->sequences);
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
@@ -299,6 +318,7 @@ int mib_scale_by(void* x, int32_t dtype, int64_t n, const float* factor, cudaStr
   if (!x || !factor) return fail(MIB_ERR_PARAM, "NULL buffer");
   if (!known_dtype(dtype)) return fail(MIB_ERR_UNSUPPORTED, "the buffer must be fp32, bf16 or fp16");
   if (n < 1) return fail(MIB_ERR_SHAPE, "empty buffer");
+  if (!aligned(x, dtype_size(dtype))) return fail(MIB_ERR_PARAM, "misaligned buffer");
   cudaError_t e = with_dtype(dtype, [&](auto v) { return mib::scale_by_t<decltype(v)>(x, n, factor, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "scale_by launch");
   return MIB_OK;
@@ -325,6 +345,8 @@ int mib_clip_grad_norm(const void* const* in, void* const* out, const int64_t* n
     if (!known_dtype(in_dtype[i]) || (out && !known_dtype(out_dtype[i])))
       return fail(MIB_ERR_UNSUPPORTED, "gradients must be fp32, bf16 or fp16");
     if (numel[i] > 0 && (!in[i] || (out && !out[i]))) return fail(MIB_ERR_PARAM, "NULL tensor");
+    if (!aligned(in[i], dtype_size(in_dtype[i])) || (out && !aligned(out[i], dtype_size(out_dtype[i]))))
+      return fail(MIB_ERR_PARAM, "misaligned tensor");
     if (out && (out[i] != in[i] || out_dtype[i] != in_dtype[i])) in_place = false;
   }
   int64_t need = 0;

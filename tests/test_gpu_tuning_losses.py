@@ -189,6 +189,21 @@ def test_policy_loss_without_tokens(cuda):
     assert tuning.token_logprobs(e, z.long()).shape == (0,)
 
 
+def test_what_stands_at_ignored_rows_is_not_read(cuda):
+    cu = [0, 20, 41, 60]
+    x, t, old, adv, ref = policy_inputs(60, 700, torch.bfloat16, 12, cu, False)
+    cul = torch.tensor(cu, device="cuda")
+    a, ga = tuning.policy_loss_grad(x, t, old, adv, ref, kl_coef=0.1, cu_seqlens=cul)
+    p, gp = tuning.preference_loss_grad(x[:41], t[:41], ref[:41], cu_seqlens=cul[:3])
+    off = t == O.IGNORE
+    for bad in (math.nan, math.inf, -math.inf, torch.finfo(torch.float32).max):
+        y, u, v, w = x.clone(), old.clone(), adv.clone(), ref.clone()
+        y[off], u[off], v[off], w[off] = bad, bad, bad, bad
+        b, gb = tuning.policy_loss_grad(y, t, u, v, w, kl_coef=0.1, cu_seqlens=cul)
+        q, gq = tuning.preference_loss_grad(y[:41], t[:41], w[:41], cu_seqlens=cul[:3])
+        assert all(torch.equal(i, j) for i, j in zip((*a, ga, *p, gp), (*b, gb, *q, gq)))
+
+
 def test_gradient_against_differences(cuda):
     """Central differences of the loss along random directions of unit length per row.  The loss is good to about
     2e-6, divided by 2h = 0.2; its third derivative along such a direction is under 1, times h^2 / 6 = 1.7e-3: 2e-3."""

@@ -34,6 +34,7 @@ def test_token_rows_are_checked():
     assert lp(_rows(logits=None)) == N.MIB_ERR_PARAM
     assert lp(_rows(targets=None)) == N.MIB_ERR_PARAM
     assert lp(_rows(logits=0x1002)) == N.MIB_ERR_PARAM                       # fp32 off its alignment
+    assert lp(_rows(targets=0x1004)) == N.MIB_ERR_PARAM                      # int64 off its alignment
     assert lp(_rows(dtype=3)) == N.MIB_ERR_UNSUPPORTED
     assert lp(_rows(rows=0)) == N.MIB_ERR_SHAPE
     assert lp(_rows(cols=0)) == N.MIB_ERR_SHAPE
@@ -91,6 +92,9 @@ def test_embedding_arguments_are_checked():
     assert g(gt=N.BF16, ot=N.F16) == N.MIB_ERR_UNSUPPORTED
     assert g(ld=7) == N.MIB_ERR_SHAPE
     assert g() == N.MIB_ERR_PARAM and b"workspace" in L.mib_last_error()
+    odd = ctypes.c_void_p(0x1002)
+    assert L.mib_embedding_lookup(FAKE, 1, 4, odd, N.F32, 9, 8, 8, 1.0, FAKE, None) == N.MIB_ERR_PARAM
+    assert L.mib_embedding_lookup(odd, 0, 4, FAKE, N.F32, 9, 8, 8, 1.0, FAKE, None) == N.MIB_ERR_PARAM
     n = N.c_i64(0)
     assert L.mib_embedding_grad_workspace(0, 9, 8, n) == N.MIB_ERR_SHAPE
     assert L.mib_embedding_grad_workspace(16384, 151936, 1024, n) == 0 and n.value > 8 * 16384
