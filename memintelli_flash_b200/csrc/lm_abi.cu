@@ -98,14 +98,12 @@ mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row, bool
   a.ignore_index = t->ignore_index;
   const double k = 1.4426950408889634 / t->temperature;
   a.k.hi = static_cast<float>(k);
-  a.k.lo = mib::kNoLow;
-  a.k.inv_hi = static_cast<float>(1.0 / t->temperature);
-  if (static_cast<double>(a.k.inv_hi) >= 1.0 / t->temperature) a.k.inv_hi = std::nextafter(a.k.inv_hi, 0.0f);
-  a.k.inv_lo = static_cast<float>(1.0 / t->temperature - static_cast<double>(a.k.inv_hi));
+  a.k.lo = 1e-30f;
   if (both) {
     if (static_cast<double>(a.k.hi) >= k) a.k.hi = std::nextafter(a.k.hi, 0.0f);
     a.k.lo = static_cast<float>(k - static_cast<double>(a.k.hi));
   }
+  a.k.k = static_cast<double>(a.k.hi) + static_cast<double>(a.k.lo);
   a.inv_temp_k = (static_cast<double>(a.k.hi) + (both ? static_cast<double>(a.k.lo) : 0.0)) * 0.6931471805599453;
   a.inv_temp = 1.0 / t->temperature;
   a.logps = logps;

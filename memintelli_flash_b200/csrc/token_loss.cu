@@ -12,8 +12,9 @@
 //
 // The maximum starts at the lowest finite float, so a row of -inf, or of the type's lowest value, needs no special
 // case: exp(-inf - m) = 0 and exp(lowest - lowest) = 1.  A row of -inf alone gives s = 0 and lp = NaN, as the
-// formula does; a NaN or +inf logit makes its row's lp NaN.  Statistics are fp32; lp is formed in double from
-// them (the difference lp - ref summed over a sequence would otherwise carry lp's fp32 rounding per token).
+// formula does; a NaN or +inf logit makes its row's lp NaN.  A thread's sums are fp32, without a mean error
+// (see Part); threads, warps and blocks are joined in double, and lp is formed in double (the difference lp - ref
+// summed over a sequence would otherwise carry each token's last rounding).
 #include "kernels.cuh"
 #include "lm_common.cuh"
 
@@ -23,29 +24,29 @@ constexpr float kLowest = -3.402823466e38f;
 
 // log2(e) / T as hi + lo.  One fp32 number is up to 6e-8 off, which every exponential of a row has in the same direction:
 // nothing next to a log-probability's own rounding, but summed over a sequence's tokens more than all their roundings.
-// So the losses use both (one operation more per element), with hi rounded down and lo above zero: -inf times lo then is
-// -inf too.  Plain log-probabilities use hi alone (lo is kNoLow: 2048 x 151936 bf16 87 us; 92 us with both), with the
-// temperature that hi stands for.
+// hi is rounded down and lo is above zero, so that -inf times either is -inf.
 struct Scale {
   float hi, lo;
-  float inv_hi, inv_lo;  // 1 / T likewise
+  double k;  // log2(e) / T
 };
-constexpr float kNoLow = 1e-30f;
-__device__ __forceinline__ Scale hi_only(Scale k) {
-  k.lo = 0.0f;
-  return k;
-}
-// exp(d / T) for joining the threads' and warps' sums.  Not by ex2: its mean error would come on top at every join.
-__device__ __forceinline__ float exp_join(float d, Scale k) { return expf(fmaf(d, k.inv_hi, d * k.inv_lo)); }
-// exp(d / T) for elements
-__device__ __forceinline__ float exp_scaled(float d, Scale k) { return ex2(fmaf(d, k.hi, d * k.lo)); }
 
-struct RowStat {
-  float m, s;
+// exp((a - b) / T) for joining a row's sums, in double: an fp32 factor's rounding would be the same in every row whose
+// differences are (16-bit logits).
+__device__ __forceinline__ double exp_of(float a, float b, Scale k) {
+  return exp2((static_cast<double>(a) - static_cast<double>(b)) * k.k);
+}
+// exp(d / T) by the hardware, within 2e-7: the gradient's elements, whose errors stay their own, and the sums' terms (see
+// Part).
+__device__ __forceinline__ float exp_hw(float d, Scale k) { return ex2(fmaf(d, k.hi, d * k.lo)); }
+
+// Maximum and sum of exponentials of a part of a row.
+struct __align__(16) RowStat {
+  double s;
+  float m;
 };
 __device__ __forceinline__ RowStat merge(RowStat a, RowStat b, Scale k) {
   const float m = fmaxf(a.m, b.m);
-  return RowStat{m, a.s * exp_join(a.m - m, k) + b.s * exp_join(b.m - m, k)};
+  return RowStat{a.s * exp_of(a.m, m, k) + b.s * exp_of(b.m, m, k), m};
 }
 
 // Elements in front of the first 16-byte boundary of a row at p (all of them when there is none).
@@ -71,6 +72,7 @@ __device__ __forceinline__ uint32_t neg_inf_word() {
   return sizeof(T) == 4 ? 0xff800000u : (std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u);
 }
 
+// The maximum of a vector's elements and m.
 template <typename T>
 __device__ __forceinline__ float vec_max(const uint4& u, float m) {
   if constexpr (sizeof(T) == 4) {
@@ -85,82 +87,113 @@ __device__ __forceinline__ float vec_max(const uint4& u, float m) {
   }
 }
 
-// The reference of a set of exponentials exp((v - m) / T).  The fast form is 2^(v k - mk) in fused operations, with mk the
-// rounded m k; `corr` (a relative correction of the results, at most 4e-4 with a square of 2e-7) makes up for that
-// rounding.  Where m k is larger (rows of a type's lowest value, say) v - m comes first: equal values give exactly 1.
-struct ExpRef {
-  float m, mk, corr;
-  bool fast;
-  __device__ __forceinline__ void set(float max, Scale k) {
-    m = max;
-    mk = max * k.hi;
-    corr = -0.6931472f * fmaf(max, k.lo, fmaf(max, k.hi, -mk));
-    fast = fabsf(mk) < 8192.0f;
-    if (!fast) corr = 0.0f;
+// How a thread adds up exponentials without a mean error.  The hardware's ex2 is low on average: by 4.95e-8 to
+// 5.1e-8 over any octave of arguments below -1, by 2.2e-8 from -1 to 0 (measured on a B200, 2^26 arguments an octave), and
+// by up to 2e-7 either way at one argument.  A sequence's tokens would add the mean up, and where logits repeat (16-bit
+// ones on a grid, flat rows) the error of the same few arguments too.  So each thread refers its terms to its maximum (or
+// more) plus an offset of its own and the row's, between 1 and 2 in units of 2's logarithm and spread evenly over the
+// threads: whatever the logits are, the arguments of a row and of all rows cover an octave below -1, the mean error is the
+// octave's, and 1 + 5.0e-8 takes it out.  The largest term is taken out too and counts as 1 exactly: a row that one logit
+// carries has no error at all.  (A polynomial in place of ex2 takes 150 us on 2048 x 151936 bf16 where this
+// takes 110, and still rounds repeated logits alike.)
+//
+// The sums keep what their additions round away: the many small terms beside a large one would each be lost, always
+// downwards (1e-8 of the row where logits spread over 30, and twice that at 32003 columns).  (Adding 16-bit logits'
+// terms in twos plainly before takes 104 us, and loses 2.5e-9 of such a row.)  What is left is within 2e-9 on average over
+// the spreads, temperatures, types and vocabularies tried.
+constexpr double kEx2Low = 5.0e-8;
+constexpr int kSums = 4, kLosts = 2;  // pairs
+constexpr float kSlack = 8.0f;        // a reference leaves room for a maximum 2^8 times as large
+struct Part {
+  float m, limit, ref;  // the maximum so far; the largest logit that `ref` has room for
+  float unit;           // of 2's logarithm
+  uint32_t place;       // the thread's, in steps near the golden section: any run of threads covers the octave evenly
+  float2 sum[kSums], lost[kLosts];
+  __device__ __forceinline__ Part(int tid, Scale k) {
+    unit = static_cast<float>(1.0 / k.k);
+    place = static_cast<uint32_t>(tid) * 5184445u;
+    restart();
+  }
+  __device__ __forceinline__ void restart() {
+    m = limit = ref = kLowest;
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) sum[i] = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kLosts; ++i) lost[i] = make_float2(0.0f, 0.0f);
+  }
+  // For logits up to `top`.
+  __device__ __forceinline__ void refer(float top) {
+    limit = top;
+    const uint32_t w = (place + (__float_as_uint(top) * 0x9e3779b1u >> 9)) & 0x7fffffu;
+    ref = top + fmaf(static_cast<float>(w), 0x1p-23f, 1.0f) * unit;
+  }
+  // The same with logits added before, and room for more.
+  __device__ __forceinline__ void raise(float top, Scale k) {
+    const float old = ref;
+    refer(top + kSlack * unit);
+    float2 any = sum[0];
+#pragma unroll
+    for (int i = 1; i < kSums; ++i) any = add2(any, sum[i]);
+    if (any.x + any.y == 0.0f) return;  // nothing yet
+    const float f = static_cast<float>(exp_of(old, ref, k));
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) sum[i] = mul2(sum[i], make_float2(f, f));
+#pragma unroll
+    for (int i = 0; i < kLosts; ++i) lost[i] = mul2(lost[i], make_float2(f, f));
+  }
+  // N vectors' elements, none above `limit`
+  template <typename T, int N>
+  __device__ __forceinline__ void add(const uint4 (&u)[N], Scale k) {
+    constexpr int P = kVec16<T> / 2;
+    const float2 minus = make_float2(-ref, -ref), hi = make_float2(k.hi, k.hi), lo = make_float2(k.lo, k.lo);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float v[kVec16<T>];
+      unpack16<T>(u[i], v);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const float2 d = add2(make_float2(v[2 * j], v[2 * j + 1]), minus), y = fma2(d, hi, mul2(d, lo));
+        const float2 e = make_float2(ex2(y.x), ex2(y.y));
+        float2 &s = sum[(i * P + j) % kSums], &l = lost[j % kLosts];
+        const float2 next = add2(s, e);
+        l = add2(l, sub2(e, sub2(next, s)));
+        s = next;
+      }
+    }
+  }
+  // The sum relative to m.  `own`: one of the terms, if there are any, is that of m itself.
+  __device__ __forceinline__ double total(bool own, Scale k) const {
+    double s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kLosts; ++i) s += static_cast<double>(lost[i].x) + static_cast<double>(lost[i].y);
+#pragma unroll
+    for (int i = 0; i < kSums; ++i) s += static_cast<double>(sum[i].x) + static_cast<double>(sum[i].y);
+    const double factor = exp_of(ref, m, k) * (1.0 + kEx2Low);
+    return own && s != 0.0 ? 1.0 + (s - static_cast<double>(exp_hw(m - ref, k))) * factor : s * factor;
   }
 };
 
-// The sum of the exponentials of N vectors' elements, as trees, corrected.
-template <typename T, bool FAST, bool LOW, int N>
-__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, Scale k) {
-  float s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    float v[kVec16<T>];
-    unpack16<T>(u[i], v);
-#pragma unroll
-    for (int e = 0; e < kVec16<T>; ++e) {
-      if (FAST) {
-        const float y = fmaf(v[e], k.hi, -r.mk);
-        v[e] = ex2(LOW ? fmaf(v[e], k.lo, y) : y);
-      } else {
-        v[e] = exp_scaled(v[e] - r.m, k);
-      }
-    }
-#pragma unroll
-    for (int w = kVec16<T> / 2; w > 0; w >>= 1)
-#pragma unroll
-      for (int e = 0; e < w; ++e) v[e] += v[e + w];
-    s += v[0];
-  }
-  return fmaf(s, r.corr, s);
-}
-template <typename T, int N>
-__device__ __forceinline__ float vecs_sum(const uint4 (&u)[N], const ExpRef& r, Scale k) {
-  if (!r.fast) return vecs_sum<T, false, true>(u, r, k);
-  return k.lo > kNoLow ? vecs_sum<T, true, true>(u, r, k) : vecs_sum<T, true, false>(u, r, k);
+// One element as a part of its own (an absent one is -inf): NaN and +inf have no sum.
+__device__ __forceinline__ RowStat one_stat(float v) {
+  return RowStat{v == -INFINITY ? 0.0 : 1.0 + static_cast<double>(v - v), fmaxf(v, kLowest)};
 }
 
-// N vectors of logits to q times their exponentials, in the logits' type.  Here k.hi is enough (the reference is set with
-// it alone): a gradient element's relative error of 1e-7 stays its own.
-template <typename T, bool FAST, int N>
-__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, Scale k, float q) {
+// N vectors of logits to q times their exponentials, in the logits' type.
+template <typename T, int N>
+__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], float m, Scale k, float q) {
+  const float2 minus = make_float2(-m, -m), hi = make_float2(k.hi, k.hi), lo = make_float2(k.lo, k.lo);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float v[kVec16<T>];
     unpack16<T>(u[i], v);
 #pragma unroll
-    for (int e = 0; e < kVec16<T>; ++e) v[e] = q * ex2(FAST ? fmaf(v[e], k.hi, -r.mk) : (v[e] - r.m) * k.hi);
+    for (int e = 0; e < kVec16<T>; e += 2) {
+      const float2 d = add2(make_float2(v[e], v[e + 1]), minus), y = fma2(d, hi, mul2(d, lo));
+      v[e] = q * ex2(y.x);
+      v[e + 1] = q * ex2(y.y);
+    }
     u[i] = pack16<T>(v);
   }
-}
-template <typename T, int N>
-__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], const ExpRef& r, Scale k, float q) {
-  if (r.fast) vecs_grad<T, true>(u, r, k, q);
-  else vecs_grad<T, false>(u, r, k, q);
-}
-
-// Mean relative error of a softmax's sum of ex2.approx results, measured on a B200 as the mean error of log-probabilities
-// against 64 bits (vocabularies of 500 to 151936, three types, two temperatures).  A sequence's tokens would add it up.
-constexpr float kEx2Mean = -2.5e-8f;
-
-// log s for s in (0, 2^127]: exponent and mantissa apart, so that the error is that of the log of a number near 1
-// (3e-8) and not half an ulp of the result (5e-7 for a vocabulary's sum).  0 gives -inf, NaN and inf themselves.
-__device__ __forceinline__ double log_sum(float s) {
-  if (!(s >= 1.1754944e-38f && s < INFINITY)) return log(static_cast<double>(s));
-  const int e = (__float_as_int(s) - 0x3f3504f3) >> 23;  // mantissa into [sqrt(1/2), sqrt(2))
-  const float f = __int_as_float(__float_as_int(s) - (e << 23));
-  return static_cast<double>(e) * 0.6931471805599453 + static_cast<double>(logf(f));
 }
 
 struct TokenArgs {
@@ -178,10 +211,7 @@ struct TokenArgs {
 
 __device__ __forceinline__ double row_logp(const TokenArgs& a, RowStat st, float target_logit, int64_t t) {
   if (t < 0 || t >= a.cols) return static_cast<double>(NAN);
-  // the largest logit's exponential is 1 exactly, the rest of the sum has the mean error
-  const float bias = kEx2Mean * (1.0f - __frcp_rn(fmaxf(st.s, 1.0f)));
-  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp_k - log_sum(st.s) +
-         static_cast<double>(bias);
+  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp_k - log(st.s);
 }
 
 // Sequence s holds rows [cu[s], cu[s + 1]); both ends are held to [0, rows] whatever the list says.
@@ -329,17 +359,20 @@ __device__ __forceinline__ float4 policy_term(const RowArgs& a, const RowScalars
 __device__ __forceinline__ void cluster_store(RowStat* p, uint32_t rank, RowStat v) {
   uint32_t to;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(to) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(to), "f"(v.m), "f"(v.s) : "memory");
+  asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(to), "d"(v.s) : "memory");
+  asm volatile("st.shared::cluster.f32 [%0+8], %1;" ::"r"(to), "f"(v.m) : "memory");
 }
 
+__device__ __forceinline__ RowStat warp_sum(double s, float m) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  return RowStat{s, m};
+}
 __device__ __forceinline__ RowStat warp_merge(RowStat t, Scale k) {
   float m = t.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float s = t.s * exp_join(t.m - m, k);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  return RowStat{m, s};
+  return warp_sum(t.s * exp_of(t.m, m, k), m);
 }
 
 // The loss and its statistics from the rows' terms, by the block that arrived last.
@@ -409,8 +442,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 
   uint4 v[NV];
   float edge = -INFINITY, coef = 0.0f;
-  RowStat st{kLowest, 0.0f};
-  ExpRef ref;
+  RowStat st{0.0, kLowest};
   if (live) {
     const uint32_t none = neg_inf_word<T>();
     if (edge_at >= 0) edge = to_f32(p[edge_at]);
@@ -425,31 +457,34 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       sc = load_scalars<T, MODE>(a, r, t);
       if (kBlock && lane == 0) shared_scalars = sc;
     }
+    Part part(tid, a.t.k);
     if constexpr (RESIDENT) {
-      st.m = fmaxf(edge, kLowest);
+      float top = kLowest;
 #pragma unroll
-      for (int u = 0; u < NV; ++u) st.m = vec_max<T>(v[u], st.m);
+      for (int u = 0; u < NV; ++u) top = vec_max<T>(v[u], top);
+      float m = fmaxf(edge, top);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) st.m = fmaxf(st.m, __shfl_xor_sync(0xffffffffu, st.m, o));
-      ref.set(st.m, a.t.k);
-      st.s = vecs_sum<T>(v, ref, a.t.k) + exp_scaled(edge - st.m, a.t.k);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      part.m = m;
+      part.refer(m);
+      part.add<T>(v, a.t.k);
+      double s = part.total(top == m, a.t.k);
+      if (edge_at >= 0) s += one_stat(edge).s * exp_of(edge, m, a.t.k);
+      st = warp_sum(s, m);
     } else {
       for (int i = 0; i < left; i += NV * GROUP) {
-        float m = st.m;
+        float top = part.m;
 #pragma unroll
         for (int u = 0; u < NV; ++u)
           v[u] = i + u * GROUP < left ? load_stream(pv + i + u * GROUP) : make_uint4(none, none, none, none);
 #pragma unroll
-        for (int u = 0; u < NV; ++u) m = vec_max<T>(v[u], m);
-        ref.set(m, a.t.k);
-        st.s = fmaf(st.s, exp_scaled(st.m - m, a.t.k), vecs_sum<T>(v, ref, a.t.k));
-        st.m = m;
+        for (int u = 0; u < NV; ++u) top = vec_max<T>(v[u], top);
+        if (top > part.limit) part.raise(top, a.t.k);
+        part.m = top;
+        part.add<T>(v, a.t.k);
       }
-      const float m = fmaxf(edge, st.m);
-      st.s = st.s * exp_join(st.m - m, a.t.k) + exp_scaled(edge - m, a.t.k);
-      st.m = m;
+      st = RowStat{part.total(true, a.t.k), part.m};
+      if (edge_at >= 0) st = merge(st, one_stat(edge), a.t.k);
       st = warp_merge(st, a.t.k);
     }
     if constexpr (kBlock) {
@@ -465,7 +500,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       }
       sc = shared_scalars;
       const int n = static_cast<int>(nranks) * kWarps;
-      st = lane < n ? stat[lane] : RowStat{kLowest, 0.0f};
+      st = lane < n ? stat[lane] : RowStat{0.0, kLowest};
       for (int i = lane + 32; i < n; i += 32) st = merge(st, stat[i], a.t.k);
       st = warp_merge(st, a.t.k);
     }
@@ -476,7 +511,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       a.t.logps[r] = static_cast<float>(lp);
       if constexpr (MODE == kPolicy) a.terms[r] = term;
       if (MODE == kStats && a.d) a.d[r] = lp - static_cast<double>(sc.ref);
-      if (MODE == kStats && a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / st.s, 0.0f, 0.0f);
+      if (MODE == kStats && a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / static_cast<float>(st.s), 0.0f, 0.0f);
     }
   } else {
     if (kBlock && nranks > 1) cluster_wait();
@@ -503,8 +538,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
     if (a.grad && have) {
       T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
       const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
-      ref.set(st.m, hi_only(a.t.k));
-      const float q0 = -coef / st.s, q = fmaf(q0, ref.corr, q0);
+      const float q = -coef / static_cast<float>(st.s);
       const bool zero = coef == 0.0f;  // zeros whatever the logits hold, NaN and infinities included
       const bool hit = t >= 0 && t < cols;
       float target_logit = 0.0f;
@@ -516,7 +550,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 #pragma unroll
           for (int u = 0; u < NV; ++u) v[u] = make_uint4(0, 0, 0, 0);
         } else {
-          vecs_grad<T>(v, ref, a.t.k, q);
+          vecs_grad<T>(v, st.m, a.t.k, q);
         }
         if (same) {
 #pragma unroll
@@ -537,11 +571,11 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
           store(i);
         }
       }
-      if (edge_at >= 0) g[edge_at] = from_f32<T>(zero ? 0.0f : q0 * exp_scaled(edge - st.m, a.t.k));
+      if (edge_at >= 0) g[edge_at] = from_f32<T>(zero ? 0.0f : q * exp_hw(edge - st.m, a.t.k));
       if (hit && !zero) {  // the target's element again, by the thread that wrote it
         const int j = static_cast<int>(t), i = (j - head) / V;
         if (j == edge_at || (j >= head && i < nvec && i >= begin && i < begin + per && (i - begin) % GROUP == tid))
-          g[j] = from_f32<T>(fmaf(q0, exp_scaled(target_logit - st.m, a.t.k), coef));
+          g[j] = from_f32<T>(fmaf(q, exp_hw(target_logit - st.m, a.t.k), coef));
       }
     }
     __syncthreads();
@@ -731,13 +765,13 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
       if (r < 0) break;
       double lp = 0.0, d = 0.0;
       float4 term = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      RowStat st{0.0f, 1.0f};
+      RowStat st{1.0, 0.0f};
       if (t != a.t.ignore_index) {
         const RowScalars sc = load_scalars<T, MODE>(a, r, t);
         const int h = static_cast<int>(live & 1);
         const bool made = mbar_wait(&stat_full[h], static_cast<uint32_t>(live >> 1) & 1, &abort_flag, kErr + 5);
         if (!__all_sync(0xffffffffu, made)) break;
-        st = warp_merge(lane < kWarps ? stat[h][lane] : RowStat{kLowest, 0.0f}, a.t.k);
+        st = warp_merge(lane < kWarps ? stat[h][lane] : RowStat{0.0, kLowest}, a.t.k);
         lp = row_logp(a.t, st, sc.target_logit, t);
         float coef = 0.0f;
         if constexpr (MODE == kPolicy) term = policy_term(a, sc, lp, coef);
@@ -745,7 +779,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         __syncwarp();
         if (lane == 0) {
           if (want_grad) {
-            row_coef = make_float4(st.m, coef, coef == 0.0f ? 0.0f : -coef / st.s, sc.target_logit);
+            row_coef = make_float4(st.m, coef, coef == 0.0f ? 0.0f : -coef / static_cast<float>(st.s), sc.target_logit);
             mbar_arrive(&coef_full);
           }
           mbar_arrive(&stat_empty[h]);
@@ -759,7 +793,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
           ++counted;
         } else {
           if (a.d) a.d[r] = d;
-          if (a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / st.s, 0.0f, 0.0f);
+          if (a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / static_cast<float>(st.s), 0.0f, 0.0f);
         }
       }
     }
@@ -771,6 +805,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
     const int tid = threadIdx.x;
     const uint32_t none = neg_inf_word<T>();
     const Scale k2 = a.t.k;
+    Part part(tid, k2);
     RingPos<SLOTS> pos;
     int64_t live = 0;
     bool ok = true;
@@ -802,9 +837,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         continue;
       }
       const float edge = edge_at >= 0 ? to_f32(p[edge_at]) : -INFINITY;
-      RowStat st{kLowest, 0.0f};
-      ExpRef ref;
-      ref.set(kLowest, k2);
+      part.restart();
       for (int c = 0; c < n && ok; ++c) {
         ok = __all_sync(0xffffffffu, mbar_wait(&full[pos.slot], pos.phase, &abort_flag, kErr + 7));
         const uint4* base = ring + pos.slot * kChunk + tid;
@@ -821,22 +854,16 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty[pos.slot]);
         }
-        // The reference follows the thread's maximum: the largest exponentials, which carry the row, are exact or nearly
-        // (a reference kept from the first part saves 5% and makes the log-probability's error three times as large).
-        float m = st.m;
+        float top = part.m;
 #pragma unroll
-        for (int u = 0; u < VECS; ++u) m = vec_max<T>(v[u], m);
-        if (m > st.m) {
-          st.s *= exp_scaled(st.m - m, k2);
-          st.m = m;
-          ref.set(m, k2);
-        }
-        st.s += vecs_sum<T>(v, ref, k2);
+        for (int u = 0; u < VECS; ++u) top = vec_max<T>(v[u], top);
+        if (top > part.limit) part.raise(top, k2);
+        part.m = top;
+        part.add<T>(v, k2);
         pos.next();
       }
-      const float m = fmaxf(edge, st.m);
-      st.s = st.s * exp_join(st.m - m, k2) + exp_scaled(edge - m, k2);
-      st.m = m;
+      RowStat st{part.total(true, k2), part.m};
+      if (edge_at >= 0) st = merge(st, one_stat(edge), k2);
       st = warp_merge(st, k2);
       const int h = static_cast<int>(live & 1);
       if (live >= 2)
@@ -853,8 +880,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
       ok = __all_sync(0xffffffffu, mbar_wait(&coef_full, static_cast<uint32_t>(live - 1) & 1, &abort_flag, kErr + 9));
       if (!ok) break;
       const float4 f = row_coef;
-      ref.set(f.x, hi_only(k2));
-      const float coef = f.y, q0 = f.z, q = fmaf(q0, ref.corr, q0);
+      const float coef = f.y, q = f.z;
       T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
       uint4* gv = reinterpret_cast<uint4*>(g + head) + tid;
       const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
@@ -880,7 +906,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         if (lane == 0) mbar_arrive(&empty[at.slot]);
         at.next();
         uint4* to = gv + static_cast<int64_t>(c) * kChunk;
-        vecs_grad<T>(v, ref, k2, q);
+        vecs_grad<T>(v, f.x, k2, q);
         if (same) {
 #pragma unroll
           for (int u = 0; u < VECS; ++u)
@@ -891,12 +917,12 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         }
       }
       if (n > keep) pos = at;
-      if (edge_at >= 0) g[edge_at] = from_f32<T>(q0 * exp_scaled(edge - f.x, k2));
+      if (edge_at >= 0) g[edge_at] = from_f32<T>(q * exp_hw(edge - f.x, k2));
       // the target's element again, by the thread that wrote it
       if (t >= 0 && t < cols) {
         const int j = static_cast<int>(t), i = (j - head) / V;
         if (j == edge_at || (j >= head && i < nvec && i % CT == tid))
-          g[j] = from_f32<T>(fmaf(q0, exp_scaled(f.w - f.x, k2), coef));
+          g[j] = from_f32<T>(fmaf(q, exp_hw(f.w - f.x, k2), coef));
       }
     }
   }
@@ -1016,12 +1042,10 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   const float c = t == a.t.ignore_index ? 0.0f : (a.slope ? a.slope[r] * static_cast<float>(a.t.inv_temp) : st.z);
   const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
   T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
-  ExpRef ref;
-  ref.set(st.x, hi_only(a.t.k));
-  const float q0 = -c * st.y, q = fmaf(q0, ref.corr, q0);
+  const float q = -c * st.y;
   const bool zero = c == 0.0f;
   float at_t = 0.0f;
-  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q0, exp_scaled(to_f32(p[t]) - st.x, a.t.k), c);
+  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q, exp_hw(to_f32(p[t]) - st.x, a.t.k), c);
   if (p == g) __syncthreads();
   const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   const int64_t head = same ? peel(g, a.t.cols) : a.t.cols;
@@ -1040,14 +1064,14 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = make_uint4(0, 0, 0, 0);
     } else {
-      vecs_grad<T>(raw, ref, a.t.k, q);
+      vecs_grad<T>(raw, st.x, a.t.k, q);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i0 + u * 256 < end) __stcs(gv + i0 + u * 256, raw[u]);
   }
   auto one = [&](int64_t j) {
-    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q0 * exp_scaled(to_f32(p[j]) - st.x, a.t.k)));
+    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q * exp_hw(to_f32(p[j]) - st.x, a.t.k)));
   };
   // the target's element again, by the thread that wrote it
   if (!zero && tv >= per * part && tv < end && (tv - per * part) % 256 == threadIdx.x) g[t] = from_f32<T>(at_t);
