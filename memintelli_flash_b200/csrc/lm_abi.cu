@@ -87,8 +87,7 @@ TokenSpace token_space(int64_t rows, int64_t sequences) {
   return s;
 }
 
-// `both`: log2(e) / T in two numbers (the losses).
-mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row, bool both) {
+mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
   mib::TokenArgs a{};
   a.logits = t->logits;
   a.map = row_map(t->layout);
@@ -96,15 +95,10 @@ mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row, bool
   a.cols = t->cols;
   a.targets = mib::IntList{t->targets, t->targets_i64};
   a.ignore_index = t->ignore_index;
-  const double k = 1.4426950408889634 / t->temperature;
-  a.k.hi = static_cast<float>(k);
-  a.k.lo = 1e-30f;
-  if (both) {
-    if (static_cast<double>(a.k.hi) >= k) a.k.hi = std::nextafter(a.k.hi, 0.0f);
-    a.k.lo = static_cast<float>(k - static_cast<double>(a.k.hi));
-  }
-  a.k.k = static_cast<double>(a.k.hi) + static_cast<double>(a.k.lo);
-  a.inv_temp_k = (static_cast<double>(a.k.hi) + (both ? static_cast<double>(a.k.lo) : 0.0)) * 0.6931471805599453;
+  a.k.k = 1.4426950408889634 / t->temperature;
+  a.k.hi = static_cast<float>(a.k.k);
+  if (static_cast<double>(a.k.hi) >= a.k.k) a.k.hi = std::nextafter(a.k.hi, 0.0f);
+  a.k.lo = static_cast<float>(a.k.k - static_cast<double>(a.k.hi));
   a.inv_temp = 1.0 / t->temperature;
   a.logps = logps;
   a.row = static_cast<float4*>(row);
@@ -195,7 +189,7 @@ int mib_token_logps(const mib_token_rows* t, float* logps, void* stats, cudaStre
   if (int r = check_token_rows(t)) return r;
   if (!logps || reinterpret_cast<uintptr_t>(stats) % 16) return fail(MIB_ERR_PARAM, "NULL or misaligned buffer");
   mib::RowArgs a{};
-  a.t = token_args(t, logps, stats, false);
+  a.t = token_args(t, logps, stats);
   cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::token_logps_t<decltype(v)>(a, stream); });
   if (e != cudaSuccess) return cuda_fail(e, "token_logps launch");
   return MIB_OK;
@@ -209,7 +203,7 @@ int mib_token_logps_grad(const mib_token_rows* t, const void* stats, const float
   if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
   if (int r = check_grad(t, grad)) return r;
   mib::GradArgs g{};
-  g.t = token_args(t, nullptr, const_cast<void*>(stats), false);
+  g.t = token_args(t, nullptr, const_cast<void*>(stats));
   g.slope = grad_logps;
   g.grad = grad;
   g.gmap = row_map(*grad_layout);
@@ -239,7 +233,7 @@ int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const 
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
   mib::RowArgs a{};
-  a.t = token_args(t, logps, nullptr, true);
+  a.t = token_args(t, logps, nullptr);
   a.seq = seq_list(t);
   a.old_logps = old_logps;
   a.advantages = advantages;
@@ -284,7 +278,7 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
   mib::RowArgs rows{};
-  rows.t = token_args(t, logps, grad ? ws + s.row : nullptr, true);
+  rows.t = token_args(t, logps, grad ? ws + s.row : nullptr);
   rows.seq = seq_list(t);
   rows.ref_logps = ref_logps;
   rows.done = reinterpret_cast<uint32_t*>(ws + s.done);

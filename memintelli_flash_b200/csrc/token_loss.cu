@@ -204,14 +204,13 @@ struct TokenArgs {
   int64_t ignore_index;
   Scale k;             // log2(e) / T
   double inv_temp;     // 1 / T
-  double inv_temp_k;   // k log(2), which the target's logit takes like the others
   float* logps;        // [rows]
   float4* row;         // [rows] {m, 1 / s, c, -}, or null
 };
 
 __device__ __forceinline__ double row_logp(const TokenArgs& a, RowStat st, float target_logit, int64_t t) {
   if (t < 0 || t >= a.cols) return static_cast<double>(NAN);
-  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp_k - log(st.s);
+  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp - log(st.s);
 }
 
 // Sequence s holds rows [cu[s], cu[s + 1]); both ends are held to [0, rows] whatever the list says.

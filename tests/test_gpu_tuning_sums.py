@@ -53,3 +53,15 @@ def test_summed_log_ratios_have_no_mean_error(vocab, dtype, cuda):
             got = rewards(x, t, ref, temperature)
             off[temperature, spread] = float((got - want).abs().max())
     assert max(off.values()) <= TOL, off
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_log_ratio_of_a_policy_to_itself_has_no_mean(dtype, cuda):
+    """``token_logprobs`` against the losses' own log-probabilities: their difference is the former's last rounding, which
+    is even over one unit in the last place: a root mean square of 1 / sqrt(12) of it."""
+    for temperature in (1.0, 0.7):
+        x, t = rows(3001, dtype, 2.5, 7)
+        old = tuning.token_logprobs(x, t, temperature=temperature)
+        unit = torch.exp2(torch.floor(torch.log2(old.double().abs())) - 23)
+        tol = TOL + 5 * (unit.square().view(2, ROWS).sum(1) / 12).sqrt()
+        assert bool((rewards(x, t, old, temperature).abs() <= tol).all())
