@@ -23,6 +23,7 @@ from .. import _native as N
 _DTYPES = {torch.float32: N.F32, torch.bfloat16: N.BF16, torch.float16: N.F16}
 _INTS = {torch.int32: 0, torch.int64: 1}
 _REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
+_PER = {None: None, "token": True, "sequence": False}
 _KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 #: loss, per-token log-probabilities, weighted KL term (without its coefficient), weighted fraction of clipped tokens
@@ -196,7 +197,7 @@ def token_logprobs(logits, targets, *, temperature=1.0, ignore_index=-100):
 
 # ---- policy loss ---------------------------------------------------------------------------------------
 def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens, reduction,
-            temperature, ignore_index, want_grad, out):
+            temperature, ignore_index, advantages_per, want_grad, out):
     rows = _Rows(logits, targets, float(temperature), int(ignore_index), cu_seqlens)
     mode = _REDUCTIONS.get(reduction)
     if mode is None:
@@ -212,8 +213,12 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_hi
         raise ValueError("the sequence mean needs a (B, T) batch or cu_seqlens")
     index, shape = rows.index, targets.shape
     old = _floats(old_logps, "old_logps", shape, index)
-    per_token = advantages.shape == shape
-    if not per_token and (rows.sequences < 1 or advantages.numel() != rows.sequences):
+    if advantages_per not in _PER:
+        raise ValueError(f'advantages_per must be "token", "sequence" or None, got {advantages_per!r}')
+    per_token = _PER[advantages_per]
+    if per_token is None:  # a list with an entry per sequence is that, even where there are as many rows
+        per_token = advantages.shape == shape and (cu_seqlens is None or len(shape) != 1 or shape[0] != rows.sequences)
+    if advantages.shape != shape if per_token else rows.sequences < 1 or advantages.numel() != rows.sequences:
         raise ValueError(f"advantages has shape {tuple(advantages.shape)}, expected {tuple(shape)} or one per sequence "
                          f"({rows.sequences})")
     adv = _floats(advantages, "advantages", advantages.shape, index)
@@ -254,27 +259,30 @@ class _LossRunc(torch.autograd.Function):
 
 
 def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=None, kl_coef=0.0,
-                cu_seqlens=None, reduction="token", temperature=1.0, ignore_index=-100):
+                cu_seqlens=None, reduction="token", temperature=1.0, ignore_index=-100, advantages_per=None):
     """Clipped policy loss with a KL term to a reference policy; returns a ``PolicyLoss``.
 
     Per token, with ``lp`` its log-probability, ``ratio = exp(lp - old_logps)`` and ``d = ref_logps - lp``:
     ``-min(ratio A, clamp(ratio, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(d) - d - 1)``.  ``reduction``: "token"
     (mean over the tokens that take part), "sequence" (mean over the sequences that have such tokens of their token
-    means) or "sum".  ``advantages``: one per token or one per sequence; ``clip_high`` defaults to ``clip_low``.
+    means) or "sum".  ``advantages``: one per token or one per sequence, as their number says, or as ``advantages_per``
+    ("token" or "sequence") does: with ``cu_seqlens`` and as many sequences as rows they are taken per sequence, which
+    differs where a sequence is empty.  ``clip_high`` defaults to ``clip_low``.
     Without a token that takes part the loss is 0."""
     def evaluate(x, want):
         return _policy(x, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens,
-                       reduction, temperature, ignore_index, want, None)
+                       reduction, temperature, ignore_index, advantages_per, want, None)
     if logits.requires_grad and torch.is_grad_enabled():
         return PolicyLoss(*_LossRunc.apply(logits, evaluate))
     return evaluate(logits, False)[0]
 
 
 def policy_loss_grad(logits, targets, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=None,
-                     kl_coef=0.0, cu_seqlens=None, reduction="token", temperature=1.0, ignore_index=-100, out=None):
+                     kl_coef=0.0, cu_seqlens=None, reduction="token", temperature=1.0, ignore_index=-100,
+                     advantages_per=None, out=None):
     """``policy_loss`` and the gradient of its loss over the logits, in their type: ``(PolicyLoss, grad)``."""
     return _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens,
-                   reduction, temperature, ignore_index, True, out)
+                   reduction, temperature, ignore_index, advantages_per, True, out)
 
 
 # ---- preference loss -----------------------------------------------------------------------------------
