@@ -275,7 +275,7 @@ int mib_row_logsumexp(const float* logits, int64_t rows, int64_t cols, int64_t l
  * hardware-aware tuning step needs around the crossbar layers.  Element types are MIB_F32, MIB_BF16 and
  * MIB_F16; arithmetic and sums are fp32 (or double where a sum is long), rounded once to the output type.
  * Index lists are int32, or int64 where the *_i64 flag is set.  Workspaces are device memory, 256-byte
- * aligned, sized by the *_workspace calls, and hold nothing between calls.
+ * aligned, sized by the *_workspace calls, and hold nothing between calls (but see mib_loss_grad).
  * ------------------------------------------------------------------------------------------------- */
 #define MIB_F32 0
 #define MIB_BF16 1
@@ -354,8 +354,12 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
                         const mib_out_layout* grad_layout, void* workspace, int64_t workspace_bytes,
                         cudaStream_t stream);
 
-/* x[i] *= *factor over n dense elements; a factor of exactly 1 leaves the buffer untouched. */
-int mib_scale_by(void* x, int32_t dtype, int64_t n, const float* factor, cudaStream_t stream);
+/* Gradient over the logits of *factor (device, NULL counts as 1) times the loss of the mib_policy_loss or
+ * mib_preference_loss call before, made with the same rows and workspace and with grad NULL: such a call leaves the rows'
+ * statistics and coefficients in the workspace until it is used again.  The factor multiplies before the only rounding
+ * to the logits' type.  `grad` as in mib_policy_loss. */
+int mib_loss_grad(const mib_token_rows* t, const void* workspace, int64_t workspace_bytes, const float* factor, void* grad,
+                  const mib_out_layout* grad_layout, cudaStream_t stream);
 
 /* Global norm of `count` dense tensors (host arrays of device addresses, sizes and types) and, when `out` is
  * non-NULL, out[i] = in[i] * min(1, max_norm / (norm + eps)); out[i] may be in[i].  norm_type is 1, 2 or 0 for

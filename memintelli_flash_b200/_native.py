@@ -108,7 +108,7 @@ _SIGS = {
                         c_i64, c_vp],
     "mib_preference_loss": [_P(TokenRows), _P(PreferenceSpec), c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, _P(OutLayout),
                             c_vp, c_i64, c_vp],
-    "mib_scale_by": [c_vp, c_i32, c_i64, c_vp, c_vp],
+    "mib_loss_grad": [_P(TokenRows), c_vp, c_i64, c_vp, c_vp, _P(OutLayout), c_vp],
     "mib_clip_grad_norm_workspace": [c_i32, _P(c_i64)],
     "mib_clip_grad_norm": [c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_f32, c_f32, c_vp, c_vp, c_i64, c_vp],
     "mib_device_status": [],

@@ -233,7 +233,7 @@ int mib_policy_loss(const mib_token_rows* t, const mib_policy_spec* spec, const 
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
   mib::RowArgs a{};
-  a.t = token_args(t, logps, nullptr);
+  a.t = token_args(t, logps, grad ? nullptr : ws + s.row);
   a.seq = seq_list(t);
   a.old_logps = old_logps;
   a.advantages = advantages;
@@ -278,7 +278,7 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
   if (int r = check_space(workspace, workspace_bytes, s.bytes)) return r;
   char* ws = static_cast<char*>(workspace);
   mib::RowArgs rows{};
-  rows.t = token_args(t, logps, grad ? ws + s.row : nullptr);
+  rows.t = token_args(t, logps, ws + s.row);
   rows.seq = seq_list(t);
   rows.ref_logps = ref_logps;
   rows.done = reinterpret_cast<uint32_t*>(ws + s.done);
@@ -306,13 +306,23 @@ int mib_preference_loss(const mib_token_rows* t, const mib_preference_spec* spec
   return MIB_OK;
 }
 
-int mib_scale_by(void* x, int32_t dtype, int64_t n, const float* factor, cudaStream_t stream) {
-  if (!x || !factor) return fail(MIB_ERR_PARAM, "NULL buffer");
-  if (!known_dtype(dtype)) return fail(MIB_ERR_UNSUPPORTED, "the buffer must be fp32, bf16 or fp16");
-  if (n < 1) return fail(MIB_ERR_SHAPE, "empty buffer");
-  if (!aligned(x, dtype_size(dtype))) return fail(MIB_ERR_PARAM, "misaligned buffer");
-  cudaError_t e = with_dtype(dtype, [&](auto v) { return mib::scale_by_t<decltype(v)>(x, n, factor, stream); });
-  if (e != cudaSuccess) return cuda_fail(e, "scale_by launch");
+int mib_loss_grad(const mib_token_rows* t, const void* workspace, int64_t workspace_bytes, const float* factor, void* grad,
+                  const mib_out_layout* grad_layout, cudaStream_t stream) {
+  if (int r = check_token_rows(t)) return r;
+  if (int r = check_sequences(t)) return r;
+  if (!grad) return fail(MIB_ERR_PARAM, "NULL buffer");
+  if (int r = check_rows_layout(grad_layout, t->rows, t->cols, "gradient")) return r;
+  if (int r = check_grad(t, grad)) return r;
+  if (!aligned(factor, 4)) return fail(MIB_ERR_PARAM, "misaligned factor");
+  const TokenSpace s = token_space(t->rows, t->sequences);
+  if (int r = check_space(const_cast<void*>(workspace), workspace_bytes, s.bytes)) return r;
+  mib::GradArgs g{};
+  g.t = token_args(t, nullptr, static_cast<char*>(const_cast<void*>(workspace)) + s.row);
+  g.factor = factor;
+  g.grad = grad;
+  g.gmap = row_map(*grad_layout);
+  cudaError_t e = with_dtype(t->dtype, [&](auto v) { return mib::logit_grad_t<decltype(v)>(g, false, stream); });
+  if (e != cudaSuccess) return cuda_fail(e, "loss_grad launch");
   return MIB_OK;
 }
 

@@ -178,9 +178,9 @@ __device__ __forceinline__ RowStat one_stat(float v) {
   return RowStat{v == -INFINITY ? 0.0 : 1.0 + static_cast<double>(v - v), fmaxf(v, kLowest)};
 }
 
-// N vectors of logits to q times their exponentials, in the logits' type.
-template <typename T, int N>
-__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], float m, Scale k, float q) {
+// N vectors of logits to q times their exponentials, and with SCALED times f, in the logits' type.
+template <typename T, bool SCALED, int N>
+__device__ __forceinline__ void vecs_grad(uint4 (&u)[N], float m, Scale k, float q, float f = 1.0f) {
   const float2 minus = make_float2(-m, -m), hi = make_float2(k.hi, k.hi), lo = make_float2(k.lo, k.lo);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -189,8 +189,10 @@ __device__ __forceinline__ void vecs_grad(uint4 (&u)[N], float m, Scale k, float
 #pragma unroll
     for (int e = 0; e < kVec16<T>; e += 2) {
       const float2 d = add2(make_float2(v[e], v[e + 1]), minus), y = fma2(d, hi, mul2(d, lo));
-      v[e] = q * ex2(y.x);
-      v[e + 1] = q * ex2(y.y);
+      float2 g = mul2(make_float2(q, q), make_float2(ex2(y.x), ex2(y.y)));
+      if (SCALED) g = mul2(g, make_float2(f, f));
+      v[e] = g.x;
+      v[e + 1] = g.y;
     }
     u[i] = pack16<T>(v);
   }
@@ -205,7 +207,7 @@ struct TokenArgs {
   Scale k;             // log2(e) / T
   double inv_temp;     // 1 / T
   float* logps;        // [rows]
-  float4* row;         // [rows] {m, 1 / s, c, -}, or null
+  float4* row;         // [rows] {m, s, c, -} for a gradient later, or null
 };
 
 __device__ __forceinline__ double row_logp(const TokenArgs& a, RowStat st, float target_logit, int64_t t) {
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       a.t.logps[r] = static_cast<float>(lp);
       if constexpr (MODE == kPolicy) a.terms[r] = term;
       if (MODE == kStats && a.d) a.d[r] = lp - static_cast<double>(sc.ref);
-      if (MODE == kStats && a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / static_cast<float>(st.s), 0.0f, 0.0f);
+      if (a.t.row) a.t.row[r] = make_float4(st.m, static_cast<float>(st.s), coef, 0.0f);
     }
   } else {
     if (kBlock && nranks > 1) cluster_wait();
@@ -519,7 +521,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       a.t.logps[r] = 0.0f;
       if constexpr (MODE == kPolicy) a.terms[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (MODE == kStats && a.d) a.d[r] = 0.0;
-      if (MODE == kStats && a.t.row) a.t.row[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
+      if (a.t.row) a.t.row[r] = make_float4(0.0f, 1.0f, 0.0f, 0.0f);
     }
   }
   if (MODE == kStats && a.done && blockIdx.x == 0 && threadIdx.x == 0) *a.done = 0;
@@ -549,7 +551,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 #pragma unroll
           for (int u = 0; u < NV; ++u) v[u] = make_uint4(0, 0, 0, 0);
         } else {
-          vecs_grad<T>(v, st.m, a.t.k, q);
+          vecs_grad<T, false>(v, st.m, a.t.k, q);
         }
         if (same) {
 #pragma unroll
@@ -763,6 +765,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
       if (lane == 0) mbar_arrive(&row_empty[b]);
       if (r < 0) break;
       double lp = 0.0, d = 0.0;
+      float coef = 0.0f;
       float4 term = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       RowStat st{1.0, 0.0f};
       if (t != a.t.ignore_index) {
@@ -772,7 +775,6 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         if (!__all_sync(0xffffffffu, made)) break;
         st = warp_merge(lane < kWarps ? stat[h][lane] : RowStat{0.0, kLowest}, a.t.k);
         lp = row_logp(a.t, st, sc.target_logit, t);
-        float coef = 0.0f;
         if constexpr (MODE == kPolicy) term = policy_term(a, sc, lp, coef);
         d = lp - static_cast<double>(sc.ref);
         __syncwarp();
@@ -792,8 +794,8 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
           ++counted;
         } else {
           if (a.d) a.d[r] = d;
-          if (a.t.row) a.t.row[r] = make_float4(st.m, 1.0f / static_cast<float>(st.s), 0.0f, 0.0f);
         }
+        if (a.t.row) a.t.row[r] = make_float4(st.m, static_cast<float>(st.s), coef, 0.0f);
       }
     }
     if (MODE == kPolicy && lane == 0) {
@@ -905,7 +907,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         if (lane == 0) mbar_arrive(&empty[at.slot]);
         at.next();
         uint4* to = gv + static_cast<int64_t>(c) * kChunk;
-        vecs_grad<T>(v, f.x, k2, q);
+        vecs_grad<T, false>(v, f.x, k2, q);
         if (same) {
 #pragma unroll
           for (int u = 0; u < VECS; ++u)
@@ -997,7 +999,7 @@ __global__ void __launch_bounds__(512) preference_pair_kernel(PreferenceArgs a) 
   }
   double loss, slope;
   preference_term(a, a.beta * (d[0] - d[1]) - a.margin, loss, slope);
-  if (a.t.row) {
+  {
     double k = slope * a.beta * a.t.inv_temp / static_cast<double>(pairs);
     if (a.average && n[side] > 0.0) k /= n[side];
     for (int64_t r = lo + tid; r < hi; r += 256) a.t.row[r].z = static_cast<float>(side ? -k : k);
@@ -1018,7 +1020,8 @@ __global__ void __launch_bounds__(512) preference_pair_kernel(PreferenceArgs a) 
 // ---- gradient of the logits from kept row statistics ---------------------------------------------------
 struct GradArgs {
   TokenArgs t;
-  const float* slope;  // [rows] d loss / d lp, or null: the coefficient is row[r].z
+  const float* slope;   // [rows] d loss / d lp, or null: the coefficient is row[r].z
+  const float* factor;  // one number that multiplies the gradient before it is rounded, or null
   void* grad;
   RowMap gmap;
   int32_t parts;       // blocks per row
@@ -1028,7 +1031,8 @@ struct GradArgs {
 //
 // `parts` blocks per row, the last rows first: the pass before read them last, and what of them is still in L2 need
 // not come from memory again.  A row whose coefficient is zero (ignored, or a flat loss) is written as zeros and not
-// read: what its logits hold does not reach the gradient.  `grad` may be the logits themselves: then one block writes
+// read: what its logits hold does not reach the gradient.  The factor multiplies each element last, so that a factor of 1
+// leaves the bits that the policy kernels write.  `grad` may be the logits themselves: then one block writes
 // a row (parts is 1), after it has read the target's logit.
 template <typename T>
 __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
@@ -1041,10 +1045,10 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   const float c = t == a.t.ignore_index ? 0.0f : (a.slope ? a.slope[r] * static_cast<float>(a.t.inv_temp) : st.z);
   const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
   T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
-  const float q = -c * st.y;
+  const float q = -c / st.y, f = a.factor ? __ldg(a.factor) : 1.0f;
   const bool zero = c == 0.0f;
   float at_t = 0.0f;
-  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q, exp_hw(to_f32(p[t]) - st.x, a.t.k), c);
+  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q, exp_hw(to_f32(p[t]) - st.x, a.t.k), c) * f;
   if (p == g) __syncthreads();
   const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   const int64_t head = same ? peel(g, a.t.cols) : a.t.cols;
@@ -1063,14 +1067,14 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
 #pragma unroll
       for (int u = 0; u < U; ++u) raw[u] = make_uint4(0, 0, 0, 0);
     } else {
-      vecs_grad<T>(raw, st.x, a.t.k, q);
+      vecs_grad<T, true>(raw, st.x, a.t.k, q, f);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (i0 + u * 256 < end) __stcs(gv + i0 + u * 256, raw[u]);
   }
   auto one = [&](int64_t j) {
-    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q * exp_hw(to_f32(p[j]) - st.x, a.t.k)));
+    g[j] = from_f32<T>(zero ? 0.0f : (j == t ? at_t : q * exp_hw(to_f32(p[j]) - st.x, a.t.k) * f));
   };
   // the target's element again, by the thread that wrote it
   if (!zero && tv >= per * part && tv < end && (tv - per * part) % 256 == threadIdx.x) g[t] = from_f32<T>(at_t);
@@ -1080,15 +1084,6 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   } else {     // rows of the two off each other's alignment
     for (int64_t j = static_cast<int64_t>(part) * 256 + threadIdx.x; j < a.t.cols; j += 256ll * a.parts) one(j);
   }
-}
-
-// x *= *factor over n elements; a factor of exactly 1 leaves the buffer untouched.
-template <typename T>
-__global__ void __launch_bounds__(256) scale_by_kernel(T* x, int64_t n, const float* __restrict__ factor) {
-  const float f = __ldg(factor);
-  if (f == 1.0f) return;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += gridDim.x * 256ll)
-    x[i] = from_f32<T>(to_f32(x[i]) * f);
 }
 
 // ---- launchers -------------------------------------------------------------------------------------
@@ -1165,15 +1160,6 @@ cudaError_t preference_loss_t(const RowArgs& rows, const PreferenceArgs& a, cons
   cudaError_t e = launch_rows<T, kStats>(rows, false, stream);
   if (e == cudaSuccess) e = launch_kernel(preference_pair_kernel, a.seq.count / 2, 512, 1, true, a, stream);
   return e != cudaSuccess || !g.grad ? e : logit_grad_t<T>(g, true, stream);
-}
-
-template <typename T>
-cudaError_t scale_by_t(void* x, int64_t n, const float* factor, cudaStream_t stream) {
-  int64_t blocks = (n + 1023) / 1024;
-  if (blocks > 148 * 8) blocks = 148 * 8;
-  scale_by_kernel<T><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<T*>(x), n, factor);
-  count_launch();
-  return cudaGetLastError();
 }
 
 }  // namespace mib

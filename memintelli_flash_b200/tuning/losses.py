@@ -7,8 +7,9 @@ row's logits are not read, its log-probability is 0 and its gradient zero.  A ta
 Sequences are the rows of a (B, T) batch of targets, or, with ``cu_seqlens`` (S + 1 non-decreasing row offsets),
 ragged ones packed in one list of rows.
 
-``policy_loss`` and ``preference_loss`` are differentiable in ``logits`` (the gradient is computed with the loss, in
-the forward call).  ``policy_loss_grad`` and ``preference_loss_grad`` return the loss and that gradient without
+``policy_loss`` and ``preference_loss`` are differentiable in ``logits``: the forward call keeps 16 bytes of each row, the
+backward call forms the gradient from them and the logits, with what multiplies the loss (a loss scale, say) before the
+gradient's only rounding to their type.  ``policy_loss_grad`` and ``preference_loss_grad`` return the loss and that gradient without
 autograd, into ``out`` if given: ``out=logits`` overwrites the logits and saves the gradient's memory.
 """
 from __future__ import annotations
@@ -225,37 +226,45 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_hi
     ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, index)
     grad, layout = rows.gradient(out) if want_grad else (None, None)
     logps, res = rows.empty(shape), rows.empty(3)
-    if rows.n == 0:
+    ws, nbytes = rows.workspace() if rows.n else (None, 0)
+    if ws is None:
         res.zero_()
     else:
-        ws, nbytes = rows.workspace()
         spec = N.PolicySpec(clip_low, clip_high, kl_coef, mode, 0 if per_token else 1)
         N.launch("mib_policy_loss", index, rows.spec, spec, old.data_ptr(), adv.data_ptr(), _address(ref), res.data_ptr(),
                  logps.data_ptr(), _address(grad), layout, ws.data_ptr(), nbytes)
     loss, kl, clipped = res.unbind(0)
-    return PolicyLoss(loss, logps, kl, clipped), grad
+    return PolicyLoss(loss, logps, kl, clipped), grad, ws
 
 
 class _LossRunc(torch.autograd.Function):
-    """A loss whose gradient over the logits was computed with it: backward scales that gradient and hands it over."""
+    """A loss that depends on each row through its log-probability: backward needs the logits and the rows' statistics and
+    coefficients, which ``evaluate`` leaves in its workspace."""
 
     @staticmethod
-    def forward(ctx, logits, evaluate):
-        result, ctx.grad = evaluate(logits, ctx.needs_input_grad[0])
+    def forward(ctx, logits, targets, cu_seqlens, temperature, ignore_index, evaluate):
+        result, ctx.space = evaluate(logits)
+        ctx.spent = False
+        ctx.save_for_backward(logits, targets, cu_seqlens)
+        ctx.args = (temperature, ignore_index)
         ctx.mark_non_differentiable(*result[1:])
         return tuple(result)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss, *_):
-        grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            raise RuntimeError("the loss's gradient was already handed over: a second backward pass needs a second "
+        space, ctx.space, spent, ctx.spent = ctx.space, None, ctx.spent, True
+        if spent:
+            raise RuntimeError("the loss's row statistics were already given back: a second backward pass needs a second "
                                "forward pass")
-        if grad.numel():
+        logits, targets, cu_seqlens = ctx.saved_tensors
+        rows = _Rows(logits, targets, *ctx.args, cu_seqlens)
+        grad, layout = rows.gradient(None)
+        if rows.n:
             factor = grad_loss.to(torch.float32).contiguous()
-            N.launch("mib_scale_by", grad.get_device(), grad.data_ptr(), _DTYPES[grad.dtype], grad.numel(), factor.data_ptr())
-        return grad, None
+            N.launch("mib_loss_grad", rows.index, rows.spec, space.data_ptr(), space.numel(), factor.data_ptr(), grad.data_ptr(),
+                     layout)
+        return grad, None, None, None, None, None
 
 
 def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=None, kl_coef=0.0,
@@ -269,12 +278,12 @@ def policy_loss(logits, targets, old_logps, advantages, ref_logps=None, *, clip_
     ("token" or "sequence") does: with ``cu_seqlens`` and as many sequences as rows they are taken per sequence, which
     differs where a sequence is empty.  ``clip_high`` defaults to ``clip_low``.
     Without a token that takes part the loss is 0."""
-    def evaluate(x, want):
+    def evaluate(x):
         return _policy(x, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens,
-                       reduction, temperature, ignore_index, advantages_per, want, None)
+                       reduction, temperature, ignore_index, advantages_per, False, None)[::2]
     if logits.requires_grad and torch.is_grad_enabled():
-        return PolicyLoss(*_LossRunc.apply(logits, evaluate))
-    return evaluate(logits, False)[0]
+        return PolicyLoss(*_LossRunc.apply(logits, targets, cu_seqlens, float(temperature), int(ignore_index), evaluate))
+    return evaluate(logits)[0]
 
 
 def policy_loss_grad(logits, targets, old_logps, advantages, ref_logps=None, *, clip_low=0.2, clip_high=None,
@@ -282,7 +291,7 @@ def policy_loss_grad(logits, targets, old_logps, advantages, ref_logps=None, *, 
                      advantages_per=None, out=None):
     """``policy_loss`` and the gradient of its loss over the logits, in their type: ``(PolicyLoss, grad)``."""
     return _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_high, kl_coef, cu_seqlens,
-                   reduction, temperature, ignore_index, advantages_per, True, out)
+                   reduction, temperature, ignore_index, advantages_per, True, out)[:2]
 
 
 # ---- preference loss -----------------------------------------------------------------------------------
@@ -311,7 +320,7 @@ def _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, m
     spec = N.PreferenceSpec(beta, label_smoothing, margin, mode, 1 if average else 0)
     N.launch("mib_preference_loss", index, rows.spec, spec, _address(ref), loss.data_ptr(), chosen.data_ptr(),
              rejected.data_ptr(), logps.data_ptr(), _address(grad), layout, ws.data_ptr(), nbytes)
-    return PreferenceLoss(loss, chosen, rejected, logps), grad
+    return PreferenceLoss(loss, chosen, rejected, logps), grad, ws
 
 
 def preference_loss(logits, targets, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0, margin=0.0,
@@ -323,16 +332,16 @@ def preference_loss(logits, targets, ref_logps=None, *, cu_seqlens=None, beta=0.
     ``h = beta (D_chosen - D_rejected) - margin``, the mean over pairs of ``kind``: "sigmoid"
     ``-(1 - e) log sigmoid(h) - e log sigmoid(-h)`` with ``e = label_smoothing``, "hinge" ``max(0, 1 - h)`` or
     "squared" ``(h - 1/2)^2``.  A sequence without a token counts as D = 0."""
-    def evaluate(x, want):
+    def evaluate(x):
         return _preference(x, targets, ref_logps, cu_seqlens, beta, label_smoothing, margin, kind, average,
-                           temperature, ignore_index, want, None)
+                           temperature, ignore_index, False, None)[::2]
     if logits.requires_grad and torch.is_grad_enabled():
-        return PreferenceLoss(*_LossRunc.apply(logits, evaluate))
-    return evaluate(logits, False)[0]
+        return PreferenceLoss(*_LossRunc.apply(logits, targets, cu_seqlens, float(temperature), int(ignore_index), evaluate))
+    return evaluate(logits)[0]
 
 
 def preference_loss_grad(logits, targets, ref_logps=None, *, cu_seqlens=None, beta=0.1, label_smoothing=0.0,
                          margin=0.0, kind="sigmoid", average=False, temperature=1.0, ignore_index=-100, out=None):
     """``preference_loss`` and the gradient of its loss over the logits, in their type: ``(PreferenceLoss, grad)``."""
     return _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, margin, kind, average,
-                       temperature, ignore_index, True, out)
+                       temperature, ignore_index, True, out)[:2]
