@@ -248,7 +248,10 @@ class _LossRunc(torch.autograd.Function):
         ctx.save_for_backward(logits, targets, cu_seqlens)
         ctx.args = (temperature, ignore_index)
         ctx.mark_non_differentiable(*result[1:])
-        return tuple(result)
+        loss = result[0]
+        if loss._is_view():  # one of several views of a buffer: autograd would refuse to change it in place
+            loss = loss.new_empty(0).set_(loss)
+        return (loss, *result[1:])
 
     @staticmethod
     @torch.autograd.function.once_differentiable

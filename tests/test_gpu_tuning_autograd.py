@@ -61,3 +61,24 @@ def test_gradients_of_strided_logits(cuda):
     g = O.policy(x[:, 3:100], u, old, adv, ref, cu=[0, 15, 30, 45, 60], **kw)[-1]
     near_grad(y.grad[:, 3:100], g, x.dtype)
     assert not y.grad[:, :3].any() and not y.grad[:, 100:].any()
+
+
+def test_the_loss_may_be_changed_in_place(cuda):
+    """``loss /= steps``, as in gradient accumulation; the other results too."""
+    cu = [0, 10, 23]
+    x, t, old, adv, ref = policy_inputs(23, 257, torch.float32, 8, cu, True)
+    kw = dict(cu_seqlens=torch.tensor(cu, device="cuda"))
+    for f, fg, args in ((tuning.policy_loss, tuning.policy_loss_grad, (old, adv, ref)),
+                        (tuning.preference_loss, tuning.preference_loss_grad, (ref,))):
+        r0, g0 = fg(x, t, *args, **kw)
+        kept = [a.clone() for a in r0]
+        y = x.clone().requires_grad_(True)
+        r = f(y, t, *args, **kw)
+        loss = r.loss
+        loss /= 4
+        loss.backward()
+        assert torch.equal(loss, kept[0] / 4) and all(torch.equal(a, b) for a, b in zip(r[1:], kept[1:]))
+        assert torch.equal(y.grad, g0 / 4)
+        for a, b in zip((*r[1:], *r0), (*kept[1:], *kept)):
+            a *= 0.5
+            assert torch.equal(a, b * 0.5)
