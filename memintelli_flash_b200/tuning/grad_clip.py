@@ -36,7 +36,7 @@ def _gradients(tensors):
         tensors = [tensors]
     grads = []
     for t in tensors:
-        if isinstance(t, torch.nn.Parameter):
+        if isinstance(t, torch.nn.Parameter) or (t.requires_grad and t.is_leaf):  # a weight: never scaled itself
             t = t.grad
             if t is None:
                 continue
@@ -87,8 +87,8 @@ def _run(grads, max_norm, norm_type, eps, out):
 
 @torch.no_grad()
 def grad_norm(tensors, norm_type=2.0):
-    """Norm (1, 2 or inf) of all gradients together, a 0-d fp32 tensor.  ``tensors``: gradients, or parameters (whose
-    ``.grad`` is taken; parameters without one are skipped)."""
+    """Norm (1, 2 or inf) of all gradients together, a 0-d fp32 tensor.  ``tensors``: gradients, or parameters and
+    other leaf tensors that require a gradient (their ``.grad`` is taken; those without one are skipped)."""
     return _run(_gradients(tensors), 0.0, norm_type, 0.0, None)
 
 
