@@ -5,6 +5,7 @@ from functools import lru_cache
 
 import torch
 import torch.nn as nn
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 
@@ -78,7 +79,7 @@ def embedding_scaled_grad(ids, grad_output, num_embeddings, scale=1.0, *, paddin
     elif not 0 <= padding_idx < num_embeddings:
         raise ValueError("padding_idx must be a row of the table")
     hidden = shape[-1]
-    ld_out, out_dtype = hidden, dtype
+    ld_out, out_dtype, given = hidden, dtype, out
     if out is None:
         if accumulate:
             raise ValueError("accumulate needs out")
@@ -106,6 +107,8 @@ def embedding_scaled_grad(ids, grad_output, num_embeddings, scale=1.0, *, paddin
     ws = g.new_empty(nbytes, dtype=torch.uint8)
     N.launch("mib_embedding_grad", index, ids.data_ptr(), wide, n, g.data_ptr(), dtype, ld, num_embeddings, hidden, scale,
              padding_idx, out.data_ptr(), out_dtype, ld_out, 1 if accumulate else 0, ws.data_ptr(), nbytes)
+    if given is not None:  # written behind autograd's back: what a graph has saved of it is gone
+        increment_version(out)
     return out
 
 

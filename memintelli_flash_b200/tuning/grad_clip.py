@@ -5,6 +5,7 @@ from array import array
 from functools import lru_cache
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 
@@ -82,6 +83,8 @@ def _run(grads, max_norm, norm_type, eps, out):
     at = lambda a: a.buffer_info()[0]  # noqa: E731
     N.launch("mib_clip_grad_norm", index, at(ptrs[0]), None if out is None else at(ptrs[-1]), at(numel), at(types[0]),
              None if out is None else at(types[-1]), len(grads), mode, max_norm, eps, norm.data_ptr(), ws.data_ptr(), nbytes)
+    if out is not None:  # written behind autograd's back: what a graph has saved of them is gone
+        increment_version(out)
     return norm
 
 

@@ -18,6 +18,7 @@ from collections import namedtuple
 from functools import lru_cache
 
 import torch
+from torch.autograd.graph import increment_version
 
 from .. import _native as N
 
@@ -233,6 +234,8 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_hi
         spec = N.PolicySpec(clip_low, clip_high, kl_coef, mode, 0 if per_token else 1)
         N.launch("mib_policy_loss", index, rows.spec, spec, old.data_ptr(), adv.data_ptr(), _address(ref), res.data_ptr(),
                  logps.data_ptr(), _address(grad), layout, ws.data_ptr(), nbytes)
+    if out is not None:  # written behind autograd's back: what a graph has saved of it is gone
+        increment_version(out)
     loss, kl, clipped = res.unbind(0)
     return PolicyLoss(loss, logps, kl, clipped), grad, ws
 
@@ -323,6 +326,8 @@ def _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, m
     spec = N.PreferenceSpec(beta, label_smoothing, margin, mode, 1 if average else 0)
     N.launch("mib_preference_loss", index, rows.spec, spec, _address(ref), loss.data_ptr(), chosen.data_ptr(),
              rejected.data_ptr(), logps.data_ptr(), _address(grad), layout, ws.data_ptr(), nbytes)
+    if out is not None:
+        increment_version(out)
     return PreferenceLoss(loss, chosen, rejected, logps), grad, ws
 
 
