@@ -289,7 +289,8 @@ int mib_embedding_lookup(const void* ids, int32_t ids_i64, int64_t n, const void
 /* Gradient of the lookup: out[v] = scale * sum over i with ids[i] = v of grad[i], in ascending i (the same bits on
  * every call); rows without a token become zero.  With accumulate the sums are added to `out` and other rows stay
  * untouched.  Tokens equal to padding_idx (-1: none) and ids outside the table add nothing.  grad (n, hidden) with
- * rows ld_grad apart; out (vocab, hidden), rows ld_out apart, of grad's type or MIB_F32. */
+ * rows ld_grad apart; out (vocab, hidden), rows ld_out apart, of grad's type or MIB_F32, apart from what is read (it is
+ * cleared first). */
 int mib_embedding_grad_workspace(int64_t n, int64_t vocab, int64_t hidden, int64_t* bytes_out);
 int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* grad, int32_t grad_dtype,
                        int64_t ld_grad, int64_t vocab, int64_t hidden, float scale, int64_t padding_idx, void* out,

@@ -92,6 +92,8 @@ def embedding_scaled_grad(ids, grad_output, num_embeddings, scale=1.0, *, paddin
             ld_out = out.stride(0)
         if hidden > 1 and out.stride(1) != 1 or ld_out < hidden:
             raise ValueError("out's rows must be dense and apart")
+        if N.overlap(out, grad_output) or N.overlap(out, ids):
+            raise ValueError("out shares memory with grad_output or ids")
     ids, wide = _check_ids(ids, index)
     n = ids.numel()
     if n == 0:

@@ -206,6 +206,20 @@ def launch(name: str, index: int, *args):
         check(rc)
 
 
+def span(t):
+    """First byte and one past the last byte that a non-empty tensor reaches."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def overlap(a, b):
+    """Whether the memory between two tensors' first and last elements has a byte in common."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 class _NoGuard:
     def __enter__(self):
         return self

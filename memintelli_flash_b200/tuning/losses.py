@@ -136,15 +136,9 @@ class _Rows:
         if a.data_ptr() == out.data_ptr():
             if a.stride() != out.stride() and self.n > 1:
                 raise ValueError("out overlaps the logits without being the same rows")
-        elif self.n and _span(a)[0] < _span(out)[1] and _span(out)[0] < _span(a)[1]:
+        elif N.overlap(a, out):
             raise ValueError("out overlaps the logits without being the same rows")
         return out, layout
-
-
-def _span(t):
-    """First byte and one past the last byte that a tensor reaches."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
 def _address(t):
