@@ -363,7 +363,8 @@ int mib_loss_grad(const mib_token_rows* t, const void* workspace, int64_t worksp
                   const mib_out_layout* grad_layout, cudaStream_t stream);
 
 /* Global norm of `count` dense tensors (host arrays of device addresses, sizes and types) and, when `out` is
- * non-NULL, out[i] = in[i] * min(1, max_norm / (norm + eps)); out[i] may be in[i].  norm_type is 1, 2 or 0 for
+ * non-NULL, out[i] = in[i] * min(1, max_norm / (norm + eps)); out[i] may be in[i], else what is written shares no memory
+ * with another tensor of the lists (refused).  norm_type is 1, 2 or 0 for
  * infinity.  *norm (device) receives the norm before clipping; a NaN or infinity among the gradients shows there and,
  * as the formula has it, in the clipped gradients. */
 int mib_clip_grad_norm_workspace(int32_t count, int64_t* bytes_out);

@@ -2,7 +2,9 @@
 // layout and launches.
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <string>
+#include <vector>
 
 #include "kernels.cuh"
 
@@ -107,6 +109,39 @@ mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
 
 mib::SeqList seq_list(const mib_token_rows* t) {
   return mib::SeqList{mib::IntList{t->cu_seqlens, t->cu_i64}, t->sequences, t->cu_seqlens ? 0 : t->rows_per_sequence};
+}
+
+// Refuses tensors of which one that is written shares memory with another that is read or written (a pair in[i], out[i]
+// may be the same tensor): the blocks that scale them run in no order.
+int check_apart(const void* const* in, void* const* out, const int64_t* numel, const int32_t* in_dtype,
+                const int32_t* out_dtype, int32_t count) {
+  struct Span {
+    uintptr_t first, end;
+    bool written;
+  };
+  std::vector<Span> spans;
+  try {
+    spans.reserve(2 * static_cast<size_t>(count));
+  } catch (const std::bad_alloc&) {
+    return fail(MIB_ERR_PARAM, "out of host memory");
+  }
+  for (int32_t i = 0; i < count; ++i) {
+    if (numel[i] == 0) continue;
+    auto add = [&](const void* p, int32_t dtype, bool written) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+      spans.push_back(Span{at, at + static_cast<uintptr_t>(numel[i]) * dtype_size(dtype), written});
+    };
+    add(out[i], out_dtype[i], true);
+    if (in[i] != out[i] || in_dtype[i] != out_dtype[i]) add(in[i], in_dtype[i], false);
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.first < b.first; });
+  uintptr_t any = 0, written = 0;  // ends of the spans so far
+  for (const Span& s : spans) {
+    if (s.first < (s.written ? any : written)) return fail(MIB_ERR_PARAM, "tensors to clip overlap in memory");
+    any = std::max(any, s.end);
+    if (s.written) written = std::max(written, s.end);
+  }
+  return MIB_OK;
 }
 
 int check_space(void* ws, int64_t have, int64_t need) {
@@ -351,6 +386,8 @@ int mib_clip_grad_norm(const void* const* in, void* const* out, const int64_t* n
       return fail(MIB_ERR_PARAM, "misaligned tensor");
     if (out && (out[i] != in[i] || out_dtype[i] != in_dtype[i])) in_place = false;
   }
+  if (out)
+    if (int r = check_apart(in, out, numel, in_dtype, out_dtype, count)) return r;
   int64_t need = 0;
   if (int r = mib_clip_grad_norm_workspace(count, &need)) return r;
   if (int r = check_space(workspace, workspace_bytes, need)) return r;
