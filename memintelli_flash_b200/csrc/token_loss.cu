@@ -694,7 +694,6 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
     abort_flag = 0;
     last = false;
     fence_mbar_init();
-    if (MODE == kStats && a.done && blockIdx.x == 0) *a.done = 0;
   }
   __syncthreads();
 
@@ -788,6 +787,8 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         ++live;
       }
       if (lane == 0) {
+        // for the next kernel; by the row, as the block of that number need not run itself
+        if (MODE == kStats && a.done && r == 0) *a.done = 0;
         a.t.logps[r] = static_cast<float>(lp);
         if constexpr (MODE == kPolicy) {
           a.terms[r] = term;
