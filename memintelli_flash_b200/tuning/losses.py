@@ -130,8 +130,7 @@ class _Rows:
         if out.shape != a.shape or out.dtype != a.dtype or out.get_device() != self.index:
             raise ValueError("out must have the logits' shape, type and device")
         layout = _layout(out)
-        if layout is None or (self.n > layout.rows_per_group and
-                              layout.group_stride < (layout.rows_per_group - 1) * layout.row_stride + out.shape[-1]):
+        if layout is None or not _apart(layout, self.n, out.shape[-1]):
             raise ValueError("out needs a unit column stride and rows that do not overlap")
         if a.data_ptr() == out.data_ptr():
             if a.stride() != out.stride() and self.n > 1:
@@ -139,6 +138,14 @@ class _Rows:
         elif N.overlap(a, out):
             raise ValueError("out overlaps the logits without being the same rows")
         return out, layout
+
+
+def _apart(layout, rows, cols):
+    """Whether no two rows of at most two levels share an element: either level may be the outer one."""
+    inner, step, jump = layout.rows_per_group, layout.row_stride, layout.group_stride
+    if rows <= inner:
+        return True
+    return jump >= (inner - 1) * step + cols or cols <= jump and step >= (rows // inner - 1) * jump + cols
 
 
 def _address(t):
