@@ -1043,13 +1043,15 @@ __global__ void __launch_bounds__(256) logit_grad_kernel(GradArgs a) {
   const int64_t t = a.t.targets[r];
   pdl_wait();
   const float4 st = __ldcg(a.t.row + r);
-  const float c = t == a.t.ignore_index ? 0.0f : (a.slope ? a.slope[r] * static_cast<float>(a.t.inv_temp) : st.z);
+  const bool in = t >= 0 && t < a.t.cols;
+  float c = t == a.t.ignore_index ? 0.0f : (a.slope ? a.slope[r] * static_cast<float>(a.t.inv_temp) : st.z);
+  if (!in && c != 0.0f) c = NAN;  // as the row's log-probability
   const T* p = static_cast<const T*>(a.t.logits) + a.t.map.at(r);
   T* g = static_cast<T*>(a.grad) + a.gmap.at(r);
   const float q = -c / st.y, f = a.factor ? __ldg(a.factor) : 1.0f;
   const bool zero = c == 0.0f;
   float at_t = 0.0f;
-  if (!zero && t >= 0 && t < a.t.cols) at_t = fmaf(q, exp_hw(to_f32(p[t]) - st.x, a.t.k), c) * f;
+  if (!zero && in) at_t = fmaf(q, exp_hw(to_f32(p[t]) - st.x, a.t.k), c) * f;
   if (p == g) __syncthreads();
   const bool same = ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(g)) & 15) == 0;
   const int64_t head = same ? peel(g, a.t.cols) : a.t.cols;
