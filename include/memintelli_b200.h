@@ -311,7 +311,7 @@ typedef struct mib_token_rows {
   mib_out_layout layout;
   int64_t ignore_index;
   int64_t sequences, rows_per_sequence;
-  double temperature;      /* log-probabilities are those of logits / temperature */
+  double temperature;      /* log-probabilities are those of logits / temperature, from 1e-30 to 1e30 */
   int32_t dtype, targets_i64, cu_i64, reserved;
 } mib_token_rows;
 

@@ -92,8 +92,8 @@ class _Rows:
             raise ValueError("logits must be (..., V) with V >= 1")
         if targets.shape != shape[:-1]:
             raise ValueError(f"targets has shape {tuple(targets.shape)}, expected {tuple(shape[:-1])}")
-        if not 0.0 < temperature < 1e30:
-            raise ValueError("temperature must be positive")
+        if not 1e-30 <= temperature < 1e30:
+            raise ValueError("temperature must be positive, from 1e-30 to 1e30")
         layout = _layout(logits)
         if layout is None:
             logits = logits.detach().contiguous()
