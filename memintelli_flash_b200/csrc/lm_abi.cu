@@ -102,6 +102,7 @@ mib::TokenArgs token_args(const mib_token_rows* t, float* logps, void* row) {
   a.k.hi = static_cast<float>(a.k.k);
   if (static_cast<double>(a.k.hi) >= a.k.k) a.k.hi = std::nextafter(a.k.hi, 0.0f);
   a.k.lo = static_cast<float>(a.k.k - static_cast<double>(a.k.hi));
+  a.k.unit = static_cast<float>(1.0 / a.k.k);
   a.inv_temp = 1.0 / t->temperature;
   a.logps = logps;
   a.row = static_cast<float4*>(row);

@@ -27,13 +27,47 @@ constexpr float kLowest = -3.402823466e38f;
 // hi is rounded down and lo is above zero, so that -inf times either is -inf.
 struct Scale {
   float hi, lo;
-  double k;  // log2(e) / T
+  double k;    // log2(e) / T
+  float unit;  // of 2's logarithm: 1 / k
 };
 
 // exp((a - b) / T) for joining a row's sums, in double: an fp32 factor's rounding would be the same in every row whose
-// differences are (16-bit logits).
+// differences are (16-bit logits).  2^x with x = n + f, |f| <= 1/2: the exponential's series at f log(2), within 1e-11.  Below
+// 2^-1000 it is 2^-1000, for a NaN too (the sums of a part that holds one are NaN by themselves).  (The library's exp2 and
+// log cost rows of 128 to 1500 fp32 logits 1 us of 10 to 20 more, by 16384 rows.)
+constexpr double kLn2 = 0.6931471805599453;
 __device__ __forceinline__ double exp_of(float a, float b, Scale k) {
-  return exp2((static_cast<double>(a) - static_cast<double>(b)) * k.k);
+  constexpr double kWhole = 6755399441055744.0;  // 1.5 * 2^52: adding it leaves n in the low bits
+  const double x = fmax((static_cast<double>(a) - static_cast<double>(b)) * k.k, -1000.0), t = x + kWhole;
+  const double r = (x - (t - kWhole)) * kLn2;
+  double p = 1.0 / 362880;
+  p = fma(r, p, 1.0 / 40320);
+  p = fma(r, p, 1.0 / 5040);
+  p = fma(r, p, 1.0 / 720);
+  p = fma(r, p, 1.0 / 120);
+  p = fma(r, p, 1.0 / 24);
+  p = fma(r, p, 1.0 / 6);
+  p = fma(r, p, 0.5);
+  p = fma(r, p, 1.0);
+  p = fma(r, p, 1.0);
+  return __hiloint2double(__double2hiint(p) + (__double2loint(t) << 20), __double2loint(p));
+}
+// log s of a row's sum: s = 2^e f with f in [sqrt(1/2), sqrt(2)), log f = 2 artanh z with z = (f - 1) / (f + 1), by its series
+// (within 1e-12).  0 gives -inf, NaN and inf themselves.
+__device__ __forceinline__ double log_of(double s) {
+  if (!(s > 1e-300 && s < 1e300)) return s > 0.0 ? s : (s == 0.0 ? -static_cast<double>(INFINITY) : s);
+  const int hi = __double2hiint(s), e = (hi - 0x3fe6a09e) >> 20;
+  const double f = __hiloint2double(hi - (e << 20), __double2loint(s)), b = f + 1.0;
+  double y = static_cast<double>(__frcp_rn(static_cast<float>(b)));
+  y *= fma(-b, y, 2.0);
+  const double z = (f - 1.0) * y, w = z * z;
+  double p = 1.0 / 13;
+  p = fma(w, p, 1.0 / 11);
+  p = fma(w, p, 1.0 / 9);
+  p = fma(w, p, 1.0 / 7);
+  p = fma(w, p, 1.0 / 5);
+  p = fma(w, p, 1.0 / 3);
+  return fma(static_cast<double>(e), kLn2, fma(z * w, 2.0 * p, 2.0 * z));
 }
 // exp(d / T) by the hardware, within 2e-7: the gradient's elements, whose errors stay their own, and the sums' terms (see
 // Part).
@@ -106,11 +140,9 @@ constexpr int kSums = 4, kLosts = 2;  // pairs
 constexpr float kSlack = 8.0f;        // a reference leaves room for a maximum 2^8 times as large
 struct Part {
   float m, limit, ref;  // the maximum so far; the largest logit that `ref` has room for
-  float unit;           // of 2's logarithm
   uint32_t place;       // the thread's, in steps near the golden section: any run of threads covers the octave evenly
   float2 sum[kSums], lost[kLosts];
-  __device__ __forceinline__ Part(int tid, Scale k) {
-    unit = static_cast<float>(1.0 / k.k);
+  __device__ __forceinline__ Part(int tid) {
     place = static_cast<uint32_t>(tid) * 5184445u;
     restart();
   }
@@ -122,15 +154,15 @@ struct Part {
     for (int i = 0; i < kLosts; ++i) lost[i] = make_float2(0.0f, 0.0f);
   }
   // For logits up to `top`.
-  __device__ __forceinline__ void refer(float top) {
+  __device__ __forceinline__ void refer(float top, Scale k) {
     limit = top;
     const uint32_t w = (place + (__float_as_uint(top) * 0x9e3779b1u >> 9)) & 0x7fffffu;
-    ref = top + fmaf(static_cast<float>(w), 0x1p-23f, 1.0f) * unit;
+    ref = top + fmaf(static_cast<float>(w), 0x1p-23f, 1.0f) * k.unit;
   }
   // The same with logits added before, and room for more.
   __device__ __forceinline__ void raise(float top, Scale k) {
     const float old = ref;
-    refer(top + kSlack * unit);
+    refer(top + kSlack * k.unit, k);
     float2 any = sum[0];
 #pragma unroll
     for (int i = 1; i < kSums; ++i) any = add2(any, sum[i]);
@@ -141,8 +173,8 @@ struct Part {
 #pragma unroll
     for (int i = 0; i < kLosts; ++i) lost[i] = mul2(lost[i], make_float2(f, f));
   }
-  // N vectors' elements, none above `limit`
-  template <typename T, int N>
+  // N vectors' elements, none above `limit`; FRESH: the first ones
+  template <typename T, bool FRESH, int N>
   __device__ __forceinline__ void add(const uint4 (&u)[N], Scale k) {
     constexpr int P = kVec16<T> / 2;
     const float2 minus = make_float2(-ref, -ref), hi = make_float2(k.hi, k.hi), lo = make_float2(k.lo, k.lo);
@@ -155,6 +187,10 @@ struct Part {
         const float2 d = add2(make_float2(v[2 * j], v[2 * j + 1]), minus), y = fma2(d, hi, mul2(d, lo));
         const float2 e = make_float2(ex2(y.x), ex2(y.y));
         float2 &s = sum[(i * P + j) % kSums], &l = lost[j % kLosts];
+        if (FRESH && i * P + j < kSums) {
+          s = e;
+          continue;
+        }
         const float2 next = add2(s, e);
         l = add2(l, sub2(e, sub2(next, s)));
         s = next;
@@ -163,11 +199,18 @@ struct Part {
   }
   // The sum relative to m.  `own`: one of the terms, if there are any, is that of m itself.
   __device__ __forceinline__ double total(bool own, Scale k) const {
-    double s = 0.0;
+    // additions in fp32 that keep their errors (each the exact rest of a sum of two), then one conversion of sum and rest
+    float2 s2 = sum[0], l = lost[0];
 #pragma unroll
-    for (int i = 0; i < kLosts; ++i) s += static_cast<double>(lost[i].x) + static_cast<double>(lost[i].y);
+    for (int i = 1; i < kSums; ++i) {
+      const float2 next = add2(s2, sum[i]), b = sub2(next, s2);
+      l = add2(l, add2(sub2(s2, sub2(next, b)), sub2(sum[i], b)));
+      s2 = next;
+    }
 #pragma unroll
-    for (int i = 0; i < kSums; ++i) s += static_cast<double>(sum[i].x) + static_cast<double>(sum[i].y);
+    for (int i = 1; i < kLosts; ++i) l = add2(l, lost[i]);
+    const float h = s2.x + s2.y, b = h - s2.x, rest = (s2.x - (h - b)) + (s2.y - b) + (l.x + l.y);
+    const double s = static_cast<double>(h) + static_cast<double>(rest);
     const double factor = exp_of(ref, m, k) * (1.0 + kEx2Low);
     return own && s != 0.0 ? 1.0 + (s - static_cast<double>(exp_hw(m - ref, k))) * factor : s * factor;
   }
@@ -212,7 +255,7 @@ struct TokenArgs {
 
 __device__ __forceinline__ double row_logp(const TokenArgs& a, RowStat st, float target_logit, int64_t t) {
   if (t < 0 || t >= a.cols) return static_cast<double>(NAN);
-  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp - log(st.s);
+  return (static_cast<double>(target_logit) - static_cast<double>(st.m)) * a.inv_temp - log_of(st.s);
 }
 
 // Sequence s holds rows [cu[s], cu[s + 1]); both ends are held to [0, rows] whatever the list says.
@@ -414,8 +457,11 @@ constexpr int kMaxCluster = 8;
 // read twice (the second time from L2, where a cluster's one row has stayed).
 //   kStats:   lp and, where asked for, m and 1 / s for a later gradient, and lp - ref
 //   kPolicy:  lp, the loss's terms, and, where asked for, the gradient
+// (A warp that reads its row twice has many loads to wait for: 8 blocks an SM, 64 registers, make the policy loss on
+// 16384 x 1500 fp32 60 us, 67 without.)
 template <typename T, int GROUP, int NV, bool RESIDENT, int MODE>
-__global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 1) token_row_kernel(RowArgs a) {
+__global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : (GROUP == 32 && !RESIDENT ? 8 : 1))
+    token_row_kernel(RowArgs a) {
   constexpr int kWarps = GROUP / 32, V = kVec16<T>;
   constexpr bool kBlock = GROUP > 32;
   __shared__ RowStat stat[kBlock ? kMaxCluster * kWarps : 1];
@@ -458,7 +504,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
       sc = load_scalars<T, MODE>(a, r, t);
       if (kBlock && lane == 0) shared_scalars = sc;
     }
-    Part part(tid, a.t.k);
+    Part part(tid);
     if constexpr (RESIDENT) {
       float top = kLowest;
 #pragma unroll
@@ -467,8 +513,8 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
       part.m = m;
-      part.refer(m);
-      part.add<T>(v, a.t.k);
+      part.refer(m, a.t.k);
+      part.add<T, true>(v, a.t.k);
       double s = part.total(top == m, a.t.k);
       if (edge_at >= 0) s += one_stat(edge).s * exp_of(edge, m, a.t.k);
       st = warp_sum(s, m);
@@ -482,7 +528,7 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
         for (int u = 0; u < NV; ++u) top = vec_max<T>(v[u], top);
         if (top > part.limit) part.raise(top, a.t.k);
         part.m = top;
-        part.add<T>(v, a.t.k);
+        part.add<T, false>(v, a.t.k);
       }
       st = RowStat{part.total(true, a.t.k), part.m};
       if (edge_at >= 0) st = merge(st, one_stat(edge), a.t.k);
@@ -807,7 +853,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
     const int tid = threadIdx.x;
     const uint32_t none = neg_inf_word<T>();
     const Scale k2 = a.t.k;
-    Part part(tid, k2);
+    Part part(tid);
     RingPos<SLOTS> pos;
     int64_t live = 0;
     bool ok = true;
@@ -861,7 +907,7 @@ __global__ void __launch_bounds__(CT + 64, CT < 512 ? 512 / CT : 1) token_ring_k
         for (int u = 0; u < VECS; ++u) top = vec_max<T>(v[u], top);
         if (top > part.limit) part.raise(top, k2);
         part.m = top;
-        part.add<T>(v, k2);
+        part.add<T, false>(v, k2);
         pos.next();
       }
       RowStat st{part.total(true, k2), part.m};
