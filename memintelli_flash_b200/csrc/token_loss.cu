@@ -642,11 +642,13 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 // front of them are given back after the statistics and copied again (from L2: the row passed moments before), while
 // the kept ones turn into gradient.  Copies of the next row start as slots fall free.
 //
-// On one B200, 1536 of 2048 rows taking part: log-probabilities of 151936 fp32 logits 140 us, 6.6 TB/s (bound by memory),
-// bf16 87 - 94 us, 5.0 - 5.3 TB/s (exponentials keep their unit busy 64% of the time); the policy loss with gradient on
-// fp32 403 us, 5.4 TB/s of the bytes it cannot do without.  Its second copies miss L2 for about a third (148 rows of
-// 608 KB are on their way; without the eviction hints 457 us).  Sharing a row between the blocks of a cluster needs no
-// second copy and measured 385 us on fp32 but 490 us on bf16, a row's exchange costing 2 us, so it is not used.
+// On one B200, 1536 of 2048 rows taking part: log-probabilities of 151936 fp32 logits 135 us, 6.9 TB/s (bound by memory),
+// bf16 106 us, 4.4 TB/s (the sums' operations: 65% of the issue slots, 55% of the multiply and of the special-function
+// pipes' cycles); the policy loss with gradient on fp32 406 us, 5.4
+// TB/s of the bytes it cannot do without, on bf16 229 us, 4.8 TB/s.  The second copies of fp32 rows miss L2 for about a
+// third (148 rows of 608 KB are on their way; without the eviction hints 457 us).  Sharing a row between the blocks of a
+// cluster needs no second copy and measured 385 us on fp32, but 490 us on 4096 rows of bf16 where this took 416, a row's
+// exchange costing 2 us, so it is not used.
 constexpr int kRowSlots = 4;  // rows between the copies and the other two
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {
@@ -1046,11 +1048,9 @@ __global__ void __launch_bounds__(512) preference_pair_kernel(PreferenceArgs a) 
   }
   double loss, slope;
   preference_term(a, a.beta * (d[0] - d[1]) - a.margin, loss, slope);
-  {
-    double k = slope * a.beta * a.t.inv_temp / static_cast<double>(pairs);
-    if (a.average && n[side] > 0.0) k /= n[side];
-    for (int64_t r = lo + tid; r < hi; r += 256) a.t.row[r].z = static_cast<float>(side ? -k : k);
-  }
+  double k = slope * a.beta * a.t.inv_temp / static_cast<double>(pairs);
+  if (a.average && n[side] > 0.0) k /= n[side];
+  for (int64_t r = lo + tid; r < hi; r += 256) a.t.row[r].z = static_cast<float>(side ? -k : k);
   if (threadIdx.x == 0) {
     a.chosen[i] = static_cast<float>(a.beta * d[0]);
     a.rejected[i] = static_cast<float>(a.beta * d[1]);
@@ -1155,14 +1155,17 @@ cudaError_t launch_ring(const RowArgs& a, bool early, cudaStream_t stream) {
   return launch_kernel(fn, a.t.rows, CT + 64, 1, early, a, stream, kSmem);
 }
 
-// The kernel for `rows` rows of `vecs` 16-byte vectors (16384 rows, log-probabilities, on one B200):
-//   up to 256 vectors   a warp per row, in registers (1000 fp32: 20 us; a block of 128 per row 35 us)
-//   up to 1024          a warp per row (with a gradient up to 400, the row then read again through the caches;
-//                       2500 fp32: 28 us; the ring 50 us)
-//   longer              the ring: blocks of 128, 4 an SM, up to 150 KB a row (64 KB rows: 83 us; blocks of 512 103 us);
-//                       of 256, 2 an SM, up to 400 KB (304 KB: 86 us; 91 us); of 512 beyond (608 KB: 139 us; 144 us)
+// The kernel for `rows` rows of `vecs` 16-byte vectors (16384 rows on one B200 where nothing else is said; "with gradient":
+// the policy loss):
+//   up to 256 vectors   a warp per row, in registers (1000 fp32: 13 us, with gradient 54; a block of 128 per row 37, 108)
+//   up to 1024          a warp per row that reads it twice (2500 fp32: 33 us; the ring 66); with gradient up to 800, as
+//                       the third reading then leaves the caches (3000 fp32: 108 us, the ring 134; 4000: 144, the ring 135;
+//                       5000 bf16: 102, the ring 171)
+//   longer              the ring: blocks of 128, 4 an SM, up to 150 KB a row (8192 rows of 64 KB: 118 us; blocks of 256 129);
+//                       of 256, 2 an SM, up to 400 KB (2048 rows of 304 KB, a quarter ignored: 106 us, with gradient 229;
+//                       blocks of 128 114, 274; of 512 107, 228); of 512 beyond (608 KB: 135 us, 411; of 256 140, 483)
 // With too few rows for one each to fill the SMs, a row goes to a block or a cluster of up to 8 blocks of 512 that
-// hold it in registers (10 vectors a thread; longer rows are read twice).
+// hold it in registers (10 vectors a thread, of which the policy kernel spills 400 bytes; longer rows are read twice).
 template <typename T, int MODE>
 cudaError_t launch_rows(const RowArgs& a, bool early, cudaStream_t stream) {
   const int64_t rows = a.t.rows, vecs = (a.t.cols + kVec16<T> - 1) / kVec16<T>;
@@ -1170,7 +1173,7 @@ cudaError_t launch_rows(const RowArgs& a, bool early, cudaStream_t stream) {
   if (vecs <= 64) return launch_kernel(token_row_kernel<T, 32, 2, true, MODE>, fours, 128, 1, early, a, stream);
   if (rows >= 192) {
     if (vecs <= 256) return launch_kernel(token_row_kernel<T, 32, 8, true, MODE>, fours, 128, 1, early, a, stream);
-    if (vecs <= (MODE == kPolicy ? 400 : 1024) && rows >= 8 * 148)
+    if (vecs <= (MODE == kPolicy ? 800 : 1024) && rows >= 8 * 148)
       return launch_kernel(token_row_kernel<T, 32, 4, false, MODE>, fours, 128, 1, early, a, stream);
     if (vecs <= 9600) return launch_ring<T, 128, 4, 6, 4, MODE>(a, early, stream);
     if (vecs <= 25600) return launch_ring<T, 256, 4, 6, 4, MODE>(a, early, stream);
