@@ -52,7 +52,8 @@ int check_token_rows(const mib_token_rows* t) {
   if (!t || !t->logits || !t->targets) return fail(MIB_ERR_PARAM, "NULL logits or targets");
   if (!known_dtype(t->dtype)) return fail(MIB_ERR_UNSUPPORTED, "logits must be fp32, bf16 or fp16");
   if (t->rows < 1 || t->cols < 1) return fail(MIB_ERR_SHAPE, "logits must be non-empty");
-  if (t->rows >= kMaxRows / 1024 || t->cols >= kMaxRows) return fail(MIB_ERR_SHAPE, "too many rows or columns");
+  if (t->rows >= kMaxRows / 1024 || t->cols >= kMaxRows)
+    return fail(MIB_ERR_SHAPE, "too many rows (2^21 or more) or columns (2^31 or more)");
   if (!(t->temperature >= 1e-30) || !(t->temperature < 1e30))  // its inverse, in fp32 too
     return fail(MIB_ERR_PARAM, "temperature must be positive, from 1e-30 to 1e30");
   if (!aligned(t->logits, dtype_size(t->dtype)) || !aligned(t->targets, index_size(t->targets_i64)) ||

@@ -3,6 +3,7 @@
 ``logits`` is (..., V), fp32, bf16 or fp16, on a CUDA device; ``targets`` holds the column of each row's token
 (shape ``logits.shape[:-1]``, int32 or int64), ``ignore_index`` where a row takes no part (prompt and padding): such a
 row's logits are not read, its log-probability is 0 and its gradient zero.  A target outside the vocabulary gives NaN.
+A call takes fewer than 2^21 rows.
 
 Sequences are the rows of a (B, T) batch of targets, or, with ``cu_seqlens`` (S + 1 non-decreasing row offsets),
 ragged ones packed in one list of rows.
