@@ -5,16 +5,16 @@
 // and every loss here depends on the logits through lp alone, so
 //   d loss / d logits[r, j] = c_r (1{j = t_r} - p[r, j]),   c_r = (d loss / d lp_r) / T.
 //
-// fp32 logits are bound by memory; 16-bit ones come near the special-function rate too (one exponential per logit and
-// pass, 16 a clock and SM).  The policy loss's coefficient belongs to one row, so its row is read once and written as
-// gradient from what is still on the chip; the preference loss's needs all rows of two sequences, so its gradient reads
-// the logits a second time.
+// fp32 logits are bound by memory; 16-bit ones by the operations of a row's sum (an exponential per logit, 16 a clock and
+// SM, and about six operations around it).  The policy loss's coefficient belongs to one row, so its row is read once and
+// written as gradient from what is still on the chip; the preference loss's needs all rows of two sequences, so its
+// gradient reads the logits a second time.
 //
 // The maximum starts at the lowest finite float, so a row of -inf, or of the type's lowest value, needs no special
 // case: exp(-inf - m) = 0 and exp(lowest - lowest) = 1.  A row of -inf alone gives s = 0 and lp = NaN, as the
-// formula does; a NaN or +inf logit makes its row's lp NaN.  A thread's sums are fp32, without a mean error
-// (see Part); threads, warps and blocks are joined in double, and lp is formed in double (the difference lp - ref
-// summed over a sequence would otherwise carry each token's last rounding).
+// formula does; a NaN or +inf logit makes its row's lp NaN.  A thread's sums are fp32, without a mean error (see Part);
+// threads, warps and blocks are joined in double, and lp is formed in double (the difference lp - ref summed over a
+// sequence would otherwise carry each token's last rounding).
 #include "kernels.cuh"
 #include "lm_common.cuh"
 
@@ -121,18 +121,18 @@ __device__ __forceinline__ float vec_max(const uint4& u, float m) {
   }
 }
 
-// How a thread adds up exponentials without a mean error.  The hardware's ex2 is low on average: by 4.95e-8 to
-// 5.1e-8 over any octave of arguments below -1, by 2.2e-8 from -1 to 0 (measured on a B200, 2^26 arguments an octave), and
-// by up to 2e-7 either way at one argument.  A sequence's tokens would add the mean up, and where logits repeat (16-bit
-// ones on a grid, flat rows) the error of the same few arguments too.  So each thread refers its terms to its maximum (or
-// more) plus an offset of its own and the row's, between 1 and 2 in units of 2's logarithm and spread evenly over the
-// threads: whatever the logits are, the arguments of a row and of all rows cover an octave below -1, the mean error is the
-// octave's, and 1 + 5.0e-8 takes it out.  The largest term is taken out too and counts as 1 exactly: a row that one logit
-// carries has no error at all.  (A polynomial in place of ex2 takes 150 us on 2048 x 151936 bf16 where this
-// takes 110, and still rounds repeated logits alike.)
+// How a thread adds up exponentials without a mean error.  The hardware's ex2 is low on average: by 4.95e-8 to 5.1e-8 over
+// any octave of arguments below -1, by 2.2e-8 from -1 to 0 (measured on a B200, 2^26 arguments an octave), and by up to 2e-7
+// either way at one argument.  A sequence's tokens would add the mean up, and where logits repeat (16-bit ones on a grid,
+// flat rows) the error of the same few arguments too.  So each thread refers its terms to its maximum (or more) plus an
+// offset of its own and the row's, between 1 and 2 in units of 2's logarithm and spread evenly over the threads: whatever
+// the logits are, the arguments of a row and of all rows cover an octave below -1, the mean error is the octave's, and
+// 1 + 5.0e-8 takes it out.  The largest term is taken out too and counts as 1 exactly: a row that one logit carries has no
+// error at all.  (A polynomial in place of ex2 takes 150 us on 2048 x 151936 bf16 where this takes 107, and still rounds
+// repeated logits alike.)
 //
 // The sums keep what their additions round away: the many small terms beside a large one would each be lost, always
-// downwards (1e-8 of the row where logits spread over 30, and twice that at 32003 columns).  (Adding 16-bit logits'
+// downwards (1e-8 of the row where logits spread over 30, and twice that at 32003 columns; 97 us).  (Adding 16-bit logits'
 // terms in twos plainly before takes 104 us, and loses 2.5e-9 of such a row.)  What is left is within 2e-9 on average over
 // the spreads, temperatures, types and vocabularies tried.
 constexpr double kEx2Low = 5.0e-8;
@@ -643,12 +643,11 @@ __global__ void __launch_bounds__(GROUP < 128 ? 128 : GROUP, GROUP == 512 ? 2 : 
 // the kept ones turn into gradient.  Copies of the next row start as slots fall free.
 //
 // On one B200, 1536 of 2048 rows taking part: log-probabilities of 151936 fp32 logits 135 us, 6.9 TB/s (bound by memory),
-// bf16 106 us, 4.4 TB/s (the sums' operations: 65% of the issue slots, 55% of the multiply and of the special-function
-// pipes' cycles); the policy loss with gradient on fp32 406 us, 5.4
-// TB/s of the bytes it cannot do without, on bf16 229 us, 4.8 TB/s.  The second copies of fp32 rows miss L2 for about a
-// third (148 rows of 608 KB are on their way; without the eviction hints 457 us).  Sharing a row between the blocks of a
-// cluster needs no second copy and measured 385 us on fp32, but 490 us on 4096 rows of bf16 where this took 416, a row's
-// exchange costing 2 us, so it is not used.
+// bf16 107 us, 4.4 TB/s (the sums' operations: 65% of the issue slots, 55% of the multiply and of the special-function
+// pipes' cycles); the policy loss with gradient on fp32 406 us, 5.4 TB/s of the bytes it cannot do without, on bf16 229 us,
+// 4.8 TB/s.  The second copies of fp32 rows miss L2 for about a third (148 rows of 608 KB are on their way; without the
+// eviction hints 457 us).  Sharing a row between the blocks of a cluster needs no second copy and measured 385 us on fp32,
+// but 490 us on 4096 rows of bf16 where this took 416, a row's exchange costing 2 us, so it is not used.
 constexpr int kRowSlots = 4;  // rows between the copies and the other two
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar, uint64_t policy) {

@@ -122,8 +122,8 @@ class _Rows:
         nbytes = _workspace_bytes(self.n, self.spec.cols, self.sequences)
         return self.logits.new_empty(nbytes, dtype=torch.uint8), nbytes
 
-    def gradient(self, out):
-        """The gradient's tensor and row addressing."""
+    def gradient(self, out, *read):
+        """The gradient's tensor and row addressing; ``read``: what the call reads beside the rows."""
         a = self.logits
         if out is None:
             out = a.new_empty(a.shape)
@@ -138,6 +138,8 @@ class _Rows:
                 raise ValueError("out overlaps the logits without being the same rows")
         elif N.overlap(a, out):
             raise ValueError("out overlaps the logits without being the same rows")
+        if any(t is not None and N.overlap(out, t) for t in (self.targets, self.cu, *read)):
+            raise ValueError("out shares memory with another argument")
         return out, layout
 
 
@@ -227,7 +229,7 @@ def _policy(logits, targets, old_logps, advantages, ref_logps, clip_low, clip_hi
                          f"({rows.sequences})")
     adv = _floats(advantages, "advantages", advantages.shape, index)
     ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, index)
-    grad, layout = rows.gradient(out) if want_grad else (None, None)
+    grad, layout = rows.gradient(out, old, adv, ref) if want_grad else (None, None)
     logps, res = rows.empty(shape), rows.empty(3)
     ws, nbytes = rows.workspace() if rows.n else (None, 0)
     if ws is None:
@@ -322,7 +324,7 @@ def _preference(logits, targets, ref_logps, cu_seqlens, beta, label_smoothing, m
         raise ValueError("preference pairs need rows")
     index, shape, pairs = rows.index, targets.shape, rows.sequences // 2
     ref = None if ref_logps is None else _floats(ref_logps, "ref_logps", shape, index)
-    grad, layout = rows.gradient(out) if want_grad else (None, None)
+    grad, layout = rows.gradient(out, ref) if want_grad else (None, None)
     logps, loss, chosen, rejected = rows.empty(shape), rows.empty(()), rows.empty(pairs), rows.empty(pairs)
     ws, nbytes = rows.workspace()
     spec = N.PreferenceSpec(beta, label_smoothing, margin, mode, 1 if average else 0)
