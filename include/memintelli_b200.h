@@ -297,9 +297,9 @@ int mib_embedding_grad(const void* ids, int32_t ids_i64, int64_t n, const void* 
                        int32_t out_dtype, int64_t ld_out, int32_t accumulate, void* workspace, int64_t workspace_bytes,
                        cudaStream_t stream);
 
-/* A (rows, cols) block of logits with a target column per row, fewer than 2^21 rows.  layout addresses rows as in mib_out_layout, with
- * col_stride 1.  Rows whose target is ignore_index take no part: their logits are not read.  A target outside
- * [0, cols) other than ignore_index makes its row's log-probability NaN.  Sequences (for entries that use them):
+/* A (rows, cols) block of logits with a target column per row, fewer than 2^21 rows.  layout addresses rows as in
+ * mib_out_layout, with col_stride 1.  Rows whose target is ignore_index take no part: their logits are not read.  A target
+ * outside [0, cols) other than ignore_index makes its row's log-probability NaN.  Sequences (for entries that use them):
  * sequence s holds rows [cu_seqlens[s], cu_seqlens[s + 1]) of a non-decreasing list of sequences + 1 offsets, or,
  * with cu_seqlens NULL, rows_per_sequence rows each; rows outside every sequence take no part in a loss (their logits
  * are not read, their log-probability is written as 0). */
